@@ -10,6 +10,7 @@
 //
 // The warps of a CTA share 16 RT weight rows and take turns along K; their sums meet in shared memory in a fixed order.
 #include "fdb_common.h"
+#include "sm100_ptx.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -23,15 +24,19 @@ struct Int4Desc {
   const void* x; void* y; const float* bias;
   const void* w; const void* scales; const void* zeros;     // packed by fdb_int4_pack; zeros may be null (8 everywhere)
   void* x_pad;                                              // [m][k rounded up to 8] when x's rows are not 16-byte aligned
+  int* status;
+  float* partial; unsigned* counter;                        // tile form with splits: [splits][m][n], one per CTA column
   long long x_ld, y_ld;
-  int dtype, scale_dtype, m, n, k, group;
+  int dtype, scale_dtype, m, n, k, group, tile_rows, splits;  // tile_rows: 0 = the vector kernel, else x rows per tile
 };
 
 struct Int4Params {
   const uint8_t* x; uint8_t* y; const float* bias;
   const uint4* w; const uint8_t* scales; const uint8_t* zeros;
+  int* status; float* partial; unsigned* counter;
   long long x_ld, y_ld;
-  int m, n, k, k_tiles, scale_kind;      // scale_kind: kF16, kBF16 or kF32
+  int m, n, k, k_tiles, splits, stages, wide;
+  uint32_t stage_bytes;
 };
 
 // ---------------------------------------------------------------------------------------------------------- packing
@@ -110,7 +115,7 @@ __global__ void int4_pad_rows(const uint16_t* __restrict__ x, uint16_t* __restri
 // ---------------------------------------------------------------------------------------------------------- product
 __device__ __forceinline__ uint4 ld_stream(const uint4* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 
@@ -118,164 +123,466 @@ template <bool BF16>
 __device__ __forceinline__ void int4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   if (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The 16-bit floats 1024 + z (fp16) or 128 + z (bf16), twice in a word.
-template <bool BF16>
-__device__ __forceinline__ uint32_t biased(uint32_t z) { return (BF16 ? 0x43004300u : 0x64006400u) | z | (z << 16); }
+// Weights as 16-bit floats. OR-ing a nibble into the low mantissa bits of 1024 (fp16) or 128 (bf16) adds it exactly;
+// fp16 also takes it four bits higher (1024 + 16 q, and a fused multiply by 1 / 16), which saves a shift.
+constexpr uint32_t kBase16 = 0x64006400u, kBaseB16 = 0x43004300u;
 
-// Nibbles p and p + 4 of a word minus the zero point, as a pair of 16-bit floats.
+// The zero point as two words: subtrahend for nibbles in the low bits, and (fp16) addend -(64 + z) for the higher ones.
+struct ZeroPair { uint32_t low, high; };
 template <bool BF16>
-__device__ __forceinline__ uint32_t weights_pair(uint32_t w, int p, uint32_t zero) {
-  const uint32_t v = ((w >> (4 * p)) & 0x000f000fu) | (BF16 ? 0x43004300u : 0x64006400u);
+__device__ __forceinline__ ZeroPair zero_pair(uint32_t z) {
+  const uint32_t zz = z * 0x00010001u;
+  if (BF16) return {kBaseB16 + zz, 0u};
+  return {kBase16 + zz, 0xd400d400u + (zz << 4)};        // -(64 + z): 0xd400 is -64, one unit of z is 16 mantissa steps
+}
+
+// The eight weights of a word, minus the zero point, as four pairs (elements 2 p and 2 p + 1 in pair p).
+template <bool BF16>
+__device__ __forceinline__ void unpack_word(uint32_t w, const ZeroPair& z, uint32_t (&out)[4]) {
   if (BF16) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&zero));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&zero));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-// SG scales of one row of a tile.
-template <int SG>
-__device__ __forceinline__ void load_scales(const Int4Params& p, long long row, float (&s)[SG]) {
-  if (p.scale_kind == kF32) {
-    const float* a = reinterpret_cast<const float*>(p.scales) + row * SG;
+    const __nv_bfloat162 zero = *reinterpret_cast<const __nv_bfloat162*>(&z.low);
 #pragma unroll
-    for (int i = 0; i < SG; ++i) s[i] = __ldg(a + i);
-    return;
-  }
-  const uint16_t* a = reinterpret_cast<const uint16_t*>(p.scales) + row * SG;
-  uint32_t w[(SG + 1) / 2];
-  if (SG == 1) {
-    w[0] = __ldg(a);
-  } else if (SG == 2) {
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(a));
-  } else if (SG == 4) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(a));
-    w[0] = v.x; w[1 % ((SG + 1) / 2)] = v.y;
+    for (int p = 0; p < 4; ++p) {
+      const uint32_t v = ((w >> (4 * p)) & 0x000f000fu) | kBaseB16;
+      const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), zero);
+      out[p] = *reinterpret_cast<const uint32_t*>(&r);
+    }
   } else {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(a));
-    w[0] = v.x; w[1 % ((SG + 1) / 2)] = v.y; w[2 % ((SG + 1) / 2)] = v.z; w[3 % ((SG + 1) / 2)] = v.w;
-  }
+    const uint32_t sixteenth = 0x2c002c00u;               // 1 / 16, twice
+    const __half2 low = *reinterpret_cast<const __half2*>(&z.low), high = *reinterpret_cast<const __half2*>(&z.high);
+    const __half2 factor = *reinterpret_cast<const __half2*>(&sixteenth);
 #pragma unroll
-  for (int i = 0; i < SG; ++i) {
-    const uint16_t h = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
-    s[i] = p.scale_kind == kBF16 ? __uint_as_float(static_cast<uint32_t>(h) << 16) : __half2float(__ushort_as_half(h));
+    for (int p = 0; p < 4; p += 2) {
+      const uint32_t x = p == 0 ? w : w >> 8;
+      const uint32_t v0 = (x & 0x000f000fu) | kBase16, v1 = (x & 0x00f000f0u) | kBase16;
+      const __half2 r0 = __hsub2(*reinterpret_cast<const __half2*>(&v0), low);
+      const __half2 r1 = __hfma2(*reinterpret_cast<const __half2*>(&v1), factor, high);
+      out[p] = *reinterpret_cast<const uint32_t*>(&r0);
+      out[p + 1] = *reinterpret_cast<const uint32_t*>(&r1);
+    }
   }
 }
 
+// SG scales of one row of a tile: fp32, or 16-bit of x's type.
+template <bool BF16, bool WIDE, int SG>
+struct ScaleRow {
+  uint32_t w[WIDE ? SG : (SG + 1) / 2];
+  __device__ __forceinline__ void load(const uint8_t* a) {
+    if (WIDE) {
+#pragma unroll
+      for (int i = 0; i < SG; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(a) + i);
+    } else if (SG == 1) {
+      w[0] = __ldg(reinterpret_cast<const uint16_t*>(a));
+    } else {
+#pragma unroll
+      for (int i = 0; i < SG / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(a) + i);
+    }
+  }
+  __device__ __forceinline__ float at(int i) const {
+    if (WIDE) return __uint_as_float(w[i]);
+    if (BF16) return __uint_as_float((i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    return __half2float(__ushort_as_half(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)))));
+  }
+};
+
 template <int SG>
-__device__ __forceinline__ uint32_t load_zeros(const Int4Params& p, long long row) {
-  if (p.zeros == nullptr) return 0x88888888u;
-  if (SG == 8) return __ldg(reinterpret_cast<const uint32_t*>(p.zeros) + row);
-  if (SG == 4) return __ldg(reinterpret_cast<const uint16_t*>(p.zeros) + row);
-  return __ldg(p.zeros + row);
+__device__ __forceinline__ uint32_t load_zeros(const uint8_t* a) {
+  if (SG == 8) return __ldg(reinterpret_cast<const uint32_t*>(a));
+  if (SG == 4) return __ldg(reinterpret_cast<const uint16_t*>(a));
+  return __ldg(a);
 }
 
 constexpr int kInt4Warps = 8;
 
-template <bool BF16, int SG, int MT, int RT>
+// Up to 8 MT rows of x; the CTA's eight warps share 16 weight rows.
+template <bool BF16, bool WIDE, bool ZERO, int SG, int MT>
 __global__ void __launch_bounds__(kInt4Warps * 32)
 int4_linear_kernel(const Int4Params p) {
-  extern __shared__ float red[];                                     // [warps][16 RT][8 MT]
+  __shared__ float red[kInt4Warps * 8 * MT * 16];
+  constexpr int kScaleBytes = 16 * SG * (WIDE ? 4 : 2), kZeroBytes = 16 * (SG >= 2 ? SG / 2 : 1);   // of a tile
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int m0 = blockIdx.y * (8 * MT);
-  const long long row_tile0 = static_cast<long long>(blockIdx.x) * RT;
-  const int row_tiles = (p.n + 15) / 16;
-  float acc[RT][MT][4] = {};
-  const uint8_t* xr[MT];
+  float acc[MT][4] = {};
+  const long long tile0 = static_cast<long long>(blockIdx.x) * p.k_tiles + warp;
+  const uint4* wp = p.w + tile0 * 64 + lane;
+  const uint8_t* sp = p.scales + tile0 * kScaleBytes + g * (kScaleBytes / 16);
+  const uint8_t* zp = ZERO ? p.zeros + tile0 * kZeroBytes + g * (kZeroBytes / 16) : nullptr;
+  const uint8_t* xp[MT];
+  bool row_in[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) xr[i] = m0 + i * 8 + g < p.m ? p.x + (m0 + i * 8 + g) * p.x_ld * 2 : nullptr;
-
-#pragma unroll(MT >= 8 ? 1 : 2)
-  for (int kt = warp; kt < p.k_tiles; kt += kInt4Warps) {
-    uint4 w[RT][2];
-    float s[RT][2][SG];
-    uint32_t z[RT][2];
+  for (int i = 0; i < MT; ++i) {
+    row_in[i] = m0 + i * 8 + g < p.m;
+    xp[i] = p.x + (row_in[i] ? (m0 + i * 8 + g) * p.x_ld * 2 : 0) + (warp * 128 + (SG == 8 ? 4 : 8) * t) * 2;
+  }
+  // Elements of x from this lane's first one to the end of the row, less those that lie ahead: a load is made when it
+  // starts inside the row (K is a multiple of 8 here, so it ends inside too).
+  int left = p.k - warp * 128 - (SG == 8 ? 4 : 8) * t;
+  // The loads of U tiles along K are in flight before the first of them is used.
+  constexpr int U = MT == 1 ? 4 : 2;
+  int todo = (p.k_tiles - warp + kInt4Warps - 1) / kInt4Warps;        // tiles of this warp
+  while (todo > 0) {
+    uint4 w[U][2];
+    ScaleRow<BF16, WIDE, SG> s[U][2];
+    uint32_t z[U][2];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const long long tile = min(row_tile0 + r, static_cast<long long>(row_tiles) - 1) * p.k_tiles + kt;
-      w[r][0] = ld_stream(p.w + tile * 64 + lane);
-      w[r][1] = ld_stream(p.w + tile * 64 + 32 + lane);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        load_scales<SG>(p, tile * 16 + g + 8 * h, s[r][h]);
-        z[r][h] = load_zeros<SG>(p, tile * 16 + g + 8 * h);
-      }
-    }
-    float part[RT][MT][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint4 xb[MT];
-      const int k = kt * 128 + j * 32;
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        xb[i] = make_uint4(0, 0, 0, 0);
-        if (SG == 8) {
-          // groups of 16: the lane's elements are 4 t .. of either group
-          if (xr[i] != nullptr) {
-            uint2 a = make_uint2(0, 0), b = make_uint2(0, 0);
-            if (k + 4 * t < p.k) a = __ldg(reinterpret_cast<const uint2*>(xr[i] + (k + 4 * t) * 2));
-            if (k + 16 + 4 * t < p.k) b = __ldg(reinterpret_cast<const uint2*>(xr[i] + (k + 16 + 4 * t) * 2));
-            xb[i] = make_uint4(a.x, a.y, b.x, b.y);
-          }
-        } else if (xr[i] != nullptr && k + 8 * t < p.k) {
-          xb[i] = __ldg(reinterpret_cast<const uint4*>(xr[i] + (k + 8 * t) * 2));
+    for (int v = 0; v < U; ++v) {
+      if (v < todo) {
+        w[v][0] = ld_stream(wp + v * kInt4Warps * 64);
+        w[v][1] = ld_stream(wp + v * kInt4Warps * 64 + 32);
+        s[v][0].load(sp + v * kInt4Warps * kScaleBytes);
+        s[v][1].load(sp + v * kInt4Warps * kScaleBytes + kScaleBytes / 2);
+        if (ZERO) {
+          z[v][0] = load_zeros<SG>(zp + v * kInt4Warps * kZeroBytes);
+          z[v][1] = load_zeros<SG>(zp + v * kInt4Warps * kZeroBytes + kZeroBytes / 2);
         }
       }
+    }
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const uint32_t wa = j == 0 ? w[r][0].x : j == 1 ? w[r][0].y : j == 2 ? w[r][0].z : w[r][0].w;
-        const uint32_t wb = j == 0 ? w[r][1].x : j == 1 ? w[r][1].y : j == 2 ? w[r][1].z : w[r][1].w;
+    for (int v = 0; v < U; ++v) {
+      if (v >= todo) break;
+      float part[MT][4];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {                                 // the two K = 16 steps of a K block of 32
+      for (int j = 0; j < 4; ++j) {
+        uint4 xb[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          xb[i] = make_uint4(0, 0, 0, 0);
+          const uint8_t* a = xp[i] + (v * kInt4Warps * 128 + j * 32) * 2;
+          const int ahead = v * kInt4Warps * 128 + j * 32;
+          if (SG == 8) {
+            // groups of 16: the lane's elements are 4 t .. of either group
+            if (row_in[i] && ahead < left) { const uint2 h = __ldg(reinterpret_cast<const uint2*>(a)); xb[i].x = h.x; xb[i].y = h.y; }
+            if (row_in[i] && ahead + 16 < left) { const uint2 h = __ldg(reinterpret_cast<const uint2*>(a + 32)); xb[i].z = h.x; xb[i].w = h.y; }
+          } else if (row_in[i] && ahead < left) {
+            xb[i] = __ldg(reinterpret_cast<const uint4*>(a));
+          }
+        }
+        const uint32_t wa = j == 0 ? w[v][0].x : j == 1 ? w[v][0].y : j == 2 ? w[v][0].z : w[v][0].w;
+        const uint32_t wb = j == 0 ? w[v][1].x : j == 1 ? w[v][1].y : j == 2 ? w[v][1].z : w[v][1].w;
+        uint32_t ra[4], rb[4];
+        const int g0 = j * 2 * SG / 8;
+        unpack_word<BF16>(wa, zero_pair<BF16>(ZERO ? (z[v][0] >> (4 * g0)) & 15u : 8u), ra);
+        unpack_word<BF16>(wb, zero_pair<BF16>(ZERO ? (z[v][1] >> (4 * g0)) & 15u : 8u), rb);
+        if (SG == 8 && ZERO) {                            // the word's second half belongs to the next group
+          uint32_t other[4];
+          unpack_word<BF16>(wa, zero_pair<BF16>((z[v][0] >> (4 * g0 + 4)) & 15u), other);
+          ra[2] = other[2]; ra[3] = other[3];
+          unpack_word<BF16>(wb, zero_pair<BF16>((z[v][1] >> (4 * g0 + 4)) & 15u), other);
+          rb[2] = other[2]; rb[3] = other[3];
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {                     // the two K = 16 steps of a K block of 32
           const int grp = (j * 2 + u) * SG / 8;
           const bool first = SG == 8 || (j * 2 + u) % (8 / SG) == 0, last = SG == 8 || (j * 2 + u + 1) % (8 / SG) == 0;
-          const uint32_t za = biased<BF16>((z[r][0] >> (4 * grp)) & 15u), zb = biased<BF16>((z[r][1] >> (4 * grp)) & 15u);
-          const uint32_t a0 = weights_pair<BF16>(wa, 2 * u, za), a2 = weights_pair<BF16>(wa, 2 * u + 1, za);
-          const uint32_t a1 = weights_pair<BF16>(wb, 2 * u, zb), a3 = weights_pair<BF16>(wb, 2 * u + 1, zb);
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
-            if (first) part[r][i][0] = part[r][i][1] = part[r][i][2] = part[r][i][3] = 0.f;
-            int4_mma<BF16>(part[r][i], a0, a1, a2, a3, u == 0 ? xb[i].x : xb[i].z, u == 0 ? xb[i].y : xb[i].w);
+            if (first) part[i][0] = part[i][1] = part[i][2] = part[i][3] = 0.f;
+            int4_mma<BF16>(part[i], ra[2 * u], rb[2 * u], ra[2 * u + 1], rb[2 * u + 1], u == 0 ? xb[i].x : xb[i].z,
+                           u == 0 ? xb[i].y : xb[i].w);
             if (last) {
-              acc[r][i][0] = fmaf(part[r][i][0], s[r][0][grp], acc[r][i][0]);
-              acc[r][i][1] = fmaf(part[r][i][1], s[r][0][grp], acc[r][i][1]);
-              acc[r][i][2] = fmaf(part[r][i][2], s[r][1][grp], acc[r][i][2]);
-              acc[r][i][3] = fmaf(part[r][i][3], s[r][1][grp], acc[r][i][3]);
+              const float s0 = s[v][0].at(grp), s1 = s[v][1].at(grp);
+              acc[i][0] = fmaf(part[i][0], s0, acc[i][0]);
+              acc[i][1] = fmaf(part[i][1], s0, acc[i][1]);
+              acc[i][2] = fmaf(part[i][2], s1, acc[i][2]);
+              acc[i][3] = fmaf(part[i][3], s1, acc[i][3]);
             }
           }
         }
       }
     }
+    todo -= U;
+    left -= U * kInt4Warps * 128;
+    wp += U * kInt4Warps * 64;
+    sp += U * kInt4Warps * kScaleBytes;
+    if (ZERO) zp += U * kInt4Warps * kZeroBytes;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) xp[i] += U * kInt4Warps * 256;
   }
-  constexpr int kRows = 16 * RT, kCols = 8 * MT;
+  constexpr int kCols = 8 * MT;
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        red[(warp * kCols + i * 8 + 2 * t + (x & 1)) * kRows + r * 16 + g + 8 * (x >> 1)] = acc[r][i][x];
+    for (int x = 0; x < 4; ++x) red[(warp * kCols + i * 8 + 2 * t + (x & 1)) * 16 + g + 8 * (x >> 1)] = acc[i][x];
   __syncthreads();
-  for (int x = threadIdx.x; x < kRows * kCols; x += blockDim.x) {
-    const int col = x / kRows, m = m0 + col;
-    const long long n = row_tile0 * 16 + x % kRows;
+  for (int x = threadIdx.x; x < 16 * kCols; x += blockDim.x) {
+    const int col = x / 16, m = m0 + col;
+    const long long n = static_cast<long long>(blockIdx.x) * 16 + x % 16;
     if (m >= p.m || n >= p.n) continue;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kInt4Warps; ++w) v += red[(w * kCols + col) * kRows + x % kRows];
+    for (int w = 0; w < kInt4Warps; ++w) v += red[(w * kCols + col) * 16 + x % 16];
     if (p.bias != nullptr) v += __ldg(p.bias + n);
     uint8_t* y = p.y + (m * p.y_ld + n) * 2;
     if (BF16) *reinterpret_cast<__nv_bfloat16*>(y) = __float2bfloat16_rn(v);
     else *reinterpret_cast<__half*>(y) = __float2half_rn(v);
   }
+}
+
+// ------------------------------------------------------------------------------------------------ more rows: tcgen05
+// From a few rows on, mma.sync (measured: 550 TFLOP/s) and the reads of x by every 16 weight rows cost more than the
+// weights' bytes. Here a CTA takes 128 weight rows as the M side of tcgen05.mma and MN rows of x as its N side:
+//   producer    bulk copies of the packed tile [128 x 128 of K] with its scales and zero points, TMA for x
+//   dequant     eight warps turn the tile into q - z in 16 bits (exact), K-major and 128B-swizzled in shared memory
+//   MMA         one product per scale group into one of four accumulators in tensor memory
+//   drain       four warps, a weight row per thread: sum += scale * accumulator, in fp32
+// so that the scales meet fp32 sums here too and the two kernels differ only in the order of their additions.
+constexpr int kTileThreads = 512;
+constexpr int kDequantWarps = 8;
+constexpr int kMaxInt4Stages = 8;
+
+template <bool BF16, int SG, int MN>
+__global__ void __launch_bounds__(kTileThreads, 1)
+int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[2 * kMaxInt4Stages + 12];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  __shared__ unsigned ticket;
+  volatile int* abort_flag = &abort_word;
+  constexpr uint32_t kX = 2 * MN * 128, kW = 8192;
+  constexpr uint32_t kZeroRow = SG >= 2 ? SG / 2 : 1;
+  const bool has_zeros = p.zeros != nullptr;
+  const uint32_t scale_row = SG * (p.wide ? 4 : 2), stage_bytes = p.stage_bytes;
+  constexpr uint32_t kTmemCols = 4 * MN < 32 ? 32 : 4 * MN;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t s_a = base, s_ring = base + 2 * 32768;
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  auto full = [&](int i) { return bar(i); };
+  auto empty = [&](int i) { return bar(kMaxInt4Stages + i); };
+  auto a_full = [&](int i) { return bar(2 * kMaxInt4Stages + i); };
+  auto a_empty = [&](int i) { return bar(2 * kMaxInt4Stages + 2 + i); };
+  auto d_full = [&](int i) { return bar(2 * kMaxInt4Stages + 4 + i); };
+  auto d_empty = [&](int i) { return bar(2 * kMaxInt4Stages + 8 + i); };
+  const int kt0 = static_cast<int>(static_cast<long long>(p.k_tiles) * blockIdx.z / p.splits);
+  const int kt1 = static_cast<int>(static_cast<long long>(p.k_tiles) * (blockIdx.z + 1) / p.splits);
+  const int n_it = kt1 - kt0;
+  const int row_tiles = (p.n + 15) / 16, rt0 = blockIdx.x * 8, rts = min(8, row_tiles - rt0);
+  const int m0 = blockIdx.y * MN;
+
+  if (tid == 0) {
+    abort_word = 0;
+    for (int i = 0; i < kMaxInt4Stages; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), kDequantWarps + 1 + 4); }
+    for (int i = 0; i < 2; ++i) { mbar_init(a_full(i), kDequantWarps); mbar_init(a_empty(i), 1); }
+    for (int i = 0; i < 4; ++i) { mbar_init(d_full(i), 1); mbar_init(d_empty(i), 4); }
+    fence_mbar_init();
+    prefetch_tensormap(&tm_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&tmem_slot), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------------------------------------- producer
+    bool ok = true;
+    int issued = 0;
+    for (int it = 0; ok && it < n_it; ++it) {
+      const int st = it % p.stages, round = it / p.stages;
+      if (round > 0) ok = mbar_wait_warp(empty(st), (round - 1) & 1, abort_flag, kStatusTimeoutProducer);
+      if (!ok) break;
+      const uint32_t at = s_ring + static_cast<uint32_t>(st) * stage_bytes;
+      const uint32_t bytes = kX + static_cast<uint32_t>(rts) * (1024 + 16 * (scale_row + (has_zeros ? kZeroRow : 0)));
+      if (lane == 0) mbar_arrive_expect_tx(full(st), bytes);
+      __syncwarp();
+      const int r = lane & 7;
+      const long long tile = static_cast<long long>(rt0 + r) * p.k_tiles + kt0 + it;
+      if (lane < 8) {
+        if (r < rts) bulk_load(at + kX + r * 1024, p.w + tile * 64, 1024, full(st));
+      } else if (lane < 16) {
+        if (r < rts) bulk_load(at + kX + kW + r * 16 * scale_row, p.scales + tile * (16 * scale_row), 16 * scale_row, full(st));
+      } else if (lane < 24) {
+        if (has_zeros && r < rts)
+          bulk_load(at + kX + kW + 128 * scale_row + r * 16 * kZeroRow, p.zeros + tile * (16 * kZeroRow), 16 * kZeroRow, full(st));
+      } else if (lane < 26) {
+        tma_load_2d(at + (lane - 24) * (MN * 128), &tm_x, full(st), (kt0 + it) * 128 + (lane - 24) * 64, m0);
+      }
+      issued = it + 1;
+    }
+    if (!ok && lane == 0) {                      // a CTA that gives up leaves no copy of its own in flight
+      for (int it = max(0, issued - p.stages); it < issued; ++it) {
+        volatile int none = 0;
+        mbar_wait(full(it % p.stages), (it / p.stages) & 1, &none, kStatusTimeoutProducer);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------------------------------------------ MMA
+    if (lane == 0) {
+      const uint32_t idesc = make_idesc(BF16 ? 1u : 0u, 128, MN);
+      bool ok = true;
+      for (int it = 0; ok && it < n_it; ++it) {
+        const int st = it % p.stages, buf = it & 1;
+        ok = mbar_wait(full(st), (it / p.stages) & 1, abort_flag, kStatusTimeoutMma) &&
+             mbar_wait(a_full(buf), (it >> 1) & 1, abort_flag, kStatusTimeoutMma);
+        const uint64_t ad = make_kmajor_desc(s_a + buf * 32768, 128);
+        const uint64_t bd = make_kmajor_desc(s_ring + static_cast<uint32_t>(st) * stage_bytes, 128);
+        for (int g = 0; ok && g < SG; ++g) {
+          const int q = it * SG + g, d = q & 3;
+          if (q >= 4) ok = mbar_wait(d_empty(d), ((q >> 2) - 1) & 1, abort_flag, kStatusTimeoutMma);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int x = 0; x < 8 / SG; ++x) {
+            const int step = g * (8 / SG) + x;
+            umma_f16(tmem + d * MN, ad + (step >> 2) * (16384 >> 4) + (step & 3) * 2,
+                     bd + (step >> 2) * ((MN * 128) >> 4) + (step & 3) * 2, idesc, x != 0 ? 1u : 0u);
+          }
+          umma_commit(d_full(d));
+        }
+        if (ok) {
+          umma_commit(a_empty(buf));
+          umma_commit(empty(st));
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 8) {
+    // -------------------------------------------------------------------------------------------------- dequant
+    const int d = warp - 8, g = lane >> 2, t = lane & 3;
+    bool ok = true;
+    for (int it = 0; ok && it < n_it; ++it) {
+      const int st = it % p.stages, buf = it & 1;
+      ok = mbar_wait_warp(full(st), (it / p.stages) & 1, abort_flag, kStatusTimeoutProducer);
+      if (ok && it >= 2) ok = mbar_wait_warp(a_empty(buf), ((it >> 1) - 1) & 1, abort_flag, kStatusTimeoutMma);
+      if (!ok) break;
+      const uint8_t* stage = smem_raw + (s_ring - smem_u32(smem_raw)) + static_cast<uint32_t>(st) * stage_bytes;
+      const uint32_t to = s_a + buf * 32768;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = d * 16 + g + 8 * h;
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + kX + d * 1024 + h * 512 + lane * 16);
+        uint32_t z = 0x88888888u;
+        if (has_zeros) {
+          const uint8_t* zr = stage + kX + kW + 128 * scale_row + row * kZeroRow;
+          z = SG == 8 ? *reinterpret_cast<const uint32_t*>(zr) : SG == 4 ? *reinterpret_cast<const uint16_t*>(zr) : *zr;
+        }
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+          // lanes of odd g take the words of a chunk in the other order: two rows' stores then meet different banks
+          const int j = jj ^ (g & 1), c = jj >> 1;
+          const uint32_t w0 = c == 0 ? v.x : v.z, w1 = c == 0 ? v.y : v.w;
+          const uint32_t word = (j & 1) ? w1 : w0;
+          const uint32_t at = to + c * 16384 + row * 128;
+          uint32_t o[4];
+          if (SG == 8) {
+            uint32_t o2[4];
+            unpack_word<BF16>(word, zero_pair<BF16>((z >> (8 * j)) & 15u), o);
+            unpack_word<BF16>(word, zero_pair<BF16>((z >> (8 * j + 4)) & 15u), o2);
+            const uint32_t unit = (j & 1) * 4 + (t >> 1);
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + ((unit ^ g) << 4) + (t & 1) * 8), "r"(o[0]), "r"(o[1]) : "memory");
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + (((unit + 2) ^ g) << 4) + (t & 1) * 8), "r"(o2[2]), "r"(o2[3]) : "memory");
+          } else {
+            const int grp = SG == 1 ? 0 : SG == 2 ? c : j;
+            unpack_word<BF16>(word, zero_pair<BF16>((z >> (4 * grp)) & 15u), o);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + ((((j & 1) * 4 + t) ^ g) << 4)), "r"(o[0]),
+                         "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(a_full(buf)); mbar_arrive(empty(st)); }
+    }
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------------------------------------------------- drain
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    float acc[MN];
+#pragma unroll
+    for (int i = 0; i < MN; ++i) acc[i] = 0.f;
+    bool ok = true;
+    for (int it = 0; ok && it < n_it; ++it) {
+      const int st = it % p.stages;
+      ok = mbar_wait_warp(full(st), (it / p.stages) & 1, abort_flag, kStatusTimeoutProducer);
+      if (!ok) break;
+      const uint8_t* sr = smem_raw + (s_ring - smem_u32(smem_raw)) + static_cast<uint32_t>(st) * stage_bytes + kX + kW + row * scale_row;
+      float s[SG];
+#pragma unroll
+      for (int g = 0; g < SG; ++g) {
+        if (p.wide) s[g] = reinterpret_cast<const float*>(sr)[g];
+        else if (BF16) s[g] = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(sr)[g]);
+        else s[g] = __half2float(reinterpret_cast<const __half*>(sr)[g]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty(st));
+#pragma unroll
+      for (int g = 0; g < SG; ++g) {
+        const int q = it * SG + g, d = q & 3;
+        ok = mbar_wait_warp(d_full(d), (q >> 2) & 1, abort_flag, kStatusTimeoutMma);
+        if (!ok) break;
+        tc_fence_after();
+        if (MN == 16) {
+          uint32_t v[16];
+          tmem_ld_32x16_wait(tmem + lanes + d * MN, v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[i] = fmaf(__uint_as_float(v[i]), s[g], acc[i]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < MN / 32; ++c) {
+            uint32_t v[32];
+            tmem_ld_32x32(tmem + lanes + d * MN + c * 32, v);
+            tmem_ld_wait_dep(v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[(c * 32 + i) % MN] = fmaf(__uint_as_float(v[i]), s[g], acc[(c * 32 + i) % MN]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(d_empty(d));
+      }
+    }
+    const long long n = static_cast<long long>(blockIdx.x) * 128 + row;
+    if (ok && n_it > 0 && p.splits == 1) {
+      const float b = p.bias != nullptr && n < p.n ? __ldg(p.bias + n) : 0.f;
+#pragma unroll
+      for (int i = 0; i < MN; ++i) {
+        if (m0 + i >= p.m || n >= p.n) continue;
+        uint8_t* y = p.y + ((m0 + i) * p.y_ld + n) * 2;
+        if (BF16) *reinterpret_cast<__nv_bfloat16*>(y) = __float2bfloat16_rn(acc[i] + b);
+        else *reinterpret_cast<__half*>(y) = __float2half_rn(acc[i] + b);
+      }
+    } else if (p.splits > 1) {
+      // the last CTA of a column to arrive adds the splits' sums in their order
+#pragma unroll
+      for (int i = 0; i < MN; ++i)
+        if (m0 + i < p.m && n < p.n) __stcg(p.partial + (static_cast<long long>(blockIdx.z) * p.m + m0 + i) * p.n + n, acc[i]);
+      __threadfence();
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const int column = blockIdx.y * gridDim.x + blockIdx.x;
+      if (warp == 4 && lane == 0) {
+        ticket = atomicAdd(p.counter + column, 1u);
+        if (ticket == static_cast<unsigned>(p.splits) - 1u) p.counter[column] = 0u;       // ready for the next launch
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (ticket == static_cast<unsigned>(p.splits) - 1u && n < p.n) {
+        __threadfence();
+        const float b = p.bias != nullptr ? __ldg(p.bias + n) : 0.f;
+        for (int i = 0; i < MN && m0 + i < p.m; ++i) {
+          float v = 0.f;
+          for (int z = 0; z < p.splits; ++z) v += __ldcg(p.partial + (static_cast<long long>(z) * p.m + m0 + i) * p.n + n);
+          uint8_t* y = p.y + ((m0 + i) * p.y_ld + n) * 2;
+          if (BF16) *reinterpret_cast<__nv_bfloat16*>(y) = __float2bfloat16_rn(v + b);
+          else *reinterpret_cast<__half*>(y) = __float2half_rn(v + b);
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (tid == 0 && abort_word != 0 && p.status != nullptr) atomicCAS(p.status, 0, abort_word);
+  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
 }
 
 }  // namespace fdb
@@ -284,32 +591,55 @@ using namespace fdb;
 
 namespace {
 
-typedef void (*Int4Kernel)(const Int4Params);
+typedef void (*Int4Tile)(const CUtensorMap, const Int4Params);
 
 template <bool BF16, int SG>
-Int4Kernel pick_rows(int mt) {
-  switch (mt) {
-    case 1: return int4_linear_kernel<BF16, SG, 1, 1>;
-    case 2: return int4_linear_kernel<BF16, SG, 2, 1>;
-    case 4: return int4_linear_kernel<BF16, SG, 4, 2>;
-    default: return int4_linear_kernel<BF16, SG, 8, 2>;
+Int4Tile pick_tile_rows(int mn) {
+  switch (mn) {
+    case 16: return int4_tile_kernel<BF16, SG, 16>;
+    case 32: return int4_tile_kernel<BF16, SG, 32>;
+    default: return int4_tile_kernel<BF16, SG, 64>;
   }
 }
 template <bool BF16>
-Int4Kernel pick(int sg, int mt) {
+Int4Tile pick_tile(int sg, int mn) {
   switch (sg) {
-    case 8: return pick_rows<BF16, 8>(mt);
-    case 4: return pick_rows<BF16, 4>(mt);
-    case 2: return pick_rows<BF16, 2>(mt);
-    default: return pick_rows<BF16, 1>(mt);
+    case 8: return pick_tile_rows<BF16, 8>(mn);
+    case 4: return pick_tile_rows<BF16, 4>(mn);
+    case 2: return pick_tile_rows<BF16, 2>(mn);
+    default: return pick_tile_rows<BF16, 1>(mn);
   }
+}
+
+typedef void (*Int4Kernel)(const Int4Params);
+
+template <bool BF16, bool WIDE, bool ZERO, int SG>
+Int4Kernel pick_rows(int mt) {
+  return mt == 1 ? int4_linear_kernel<BF16, WIDE, ZERO, SG, 1> : int4_linear_kernel<BF16, WIDE, ZERO, SG, 2>;
+}
+template <bool BF16, bool WIDE, bool ZERO>
+Int4Kernel pick_group(int sg, int mt) {
+  switch (sg) {
+    case 8: return pick_rows<BF16, WIDE, ZERO, 8>(mt);
+    case 4: return pick_rows<BF16, WIDE, ZERO, 4>(mt);
+    case 2: return pick_rows<BF16, WIDE, ZERO, 2>(mt);
+    default: return pick_rows<BF16, WIDE, ZERO, 1>(mt);
+  }
+}
+template <bool BF16>
+Int4Kernel pick(bool wide, bool zero, int sg, int mt) {
+  if (wide) return zero ? pick_group<BF16, true, true>(sg, mt) : pick_group<BF16, true, false>(sg, mt);
+  return zero ? pick_group<BF16, false, true>(sg, mt) : pick_group<BF16, false, false>(sg, mt);
 }
 
 struct Int4Op : Op {
   Int4Params p{};
   Int4Kernel kernel = nullptr;
+  Int4Tile tile = nullptr;               // set for the tile form
+  CUtensorMap tm_x;
+  int smem = 0;
   dim3 grid;
-  int smem = 0, device = 0, k8 = 0;
+  int device = 0, k8 = 0;
   const uint16_t* x_src = nullptr;        // set when x goes through x_pad
   uint16_t* x_pad = nullptr;
   long long x_src_ld = 0;
@@ -318,7 +648,8 @@ struct Int4Op : Op {
     cudaGetDevice(&at);
     if (at != device) cudaSetDevice(device);
     if (x_pad != nullptr) int4_pad_rows<<<dim3((k8 + 255) / 256, p.m), 256, 0, s>>>(x_src, x_pad, x_src_ld, p.k, k8);
-    kernel<<<grid, kInt4Warps * 32, smem, s>>>(p);
+    if (tile != nullptr) tile<<<grid, kTileThreads, smem, s>>>(tm_x, p);
+    else kernel<<<grid, kInt4Warps * 32, 0, s>>>(p);
     const cudaError_t e = cudaGetLastError();
     if (at != device) cudaSetDevice(at);
     if (e != cudaSuccess) { set_error(std::string("int4 linear: ") + cudaGetErrorString(e)); return -1; }
@@ -364,7 +695,7 @@ FDB_API int fdb_int4_pack(const void* q, const void* scales, const void* zeros, 
 FDB_API void* fdb_int4_linear_create(const Int4Desc* d) {
   auto fail = [](const std::string& what) -> void* { set_error("int4 linear: " + what); return nullptr; };
   if (d->dtype != kF16 && d->dtype != kBF16) return fail("x and y must be fp16 or bf16");
-  if (d->scale_dtype != kF16 && d->scale_dtype != kBF16 && d->scale_dtype != kF32) return fail("scales must be fp16, bf16 or fp32");
+  if (d->scale_dtype != d->dtype && d->scale_dtype != kF32) return fail("scales must be fp32 or of x's type");
   if (!group_ok(d->group)) return fail("the group size must be 16, 32, 64, 128 or 256");
   if (d->m < 1 || d->n < 1 || d->k < 1) return fail("empty sizes");
   if (d->x_ld < d->k || d->y_ld < d->n) return fail("row pitches shorter than a row");
@@ -383,17 +714,42 @@ FDB_API void* fdb_int4_linear_create(const Int4Desc* d) {
   p.y = static_cast<uint8_t*>(d->y); p.y_ld = d->y_ld; p.bias = d->bias;
   p.w = static_cast<const uint4*>(d->w); p.scales = static_cast<const uint8_t*>(d->scales);
   p.zeros = static_cast<const uint8_t*>(d->zeros);
-  p.m = d->m; p.n = d->n; p.k_tiles = (d->k + 127) / 128; p.scale_kind = d->scale_dtype;
-  const int mt = d->m <= 8 ? 1 : d->m <= 16 ? 2 : d->m <= 32 ? 4 : 8, rt = mt >= 4 ? 2 : 1;
+  p.m = d->m; p.n = d->n; p.k_tiles = (d->k + 127) / 128;
+  p.status = d->status;
   const int sg = 128 / std::min(d->group, 128);
-  op->kernel = d->dtype == kBF16 ? pick<true>(sg, mt) : pick<false>(sg, mt);
-  op->smem = kInt4Warps * 16 * rt * 8 * mt * 4;
-  const int row_tiles = (d->n + 15) / 16;
-  op->grid = dim3((row_tiles + rt - 1) / rt, (d->m + 8 * mt - 1) / (8 * mt));
-  if (op->grid.y > 65535) { delete op; return fail("too many rows"); }
-  if (op->smem > 48 * 1024 &&
-      cudaFuncSetAttribute(reinterpret_cast<const void*>(op->kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, op->smem) != cudaSuccess) {
-    cudaGetLastError(); delete op; return fail("cannot raise the dynamic shared memory limit");
+  const bool wide = d->scale_dtype == kF32, zero = d->zeros != nullptr;
+  if (d->tile_rows == 0) {
+    const int mt = d->m <= 8 ? 1 : 2;
+    op->kernel = d->dtype == kBF16 ? pick<true>(wide, zero, sg, mt) : pick<false>(wide, zero, sg, mt);
+    op->grid = dim3((d->n + 15) / 16, (d->m + 8 * mt - 1) / (8 * mt));
+  } else {
+    const int mn = d->tile_rows;
+    if ((mn != 16 && mn != 32 && mn != 64) || d->splits < 1 || d->splits > p.k_tiles ||
+        (d->splits > 1 && (d->partial == nullptr || d->counter == nullptr))) {
+      delete op; return fail("bad tile form");
+    }
+    p.splits = d->splits; p.partial = d->partial; p.counter = d->counter;
+    op->tile = d->dtype == kBF16 ? pick_tile<true>(sg, mn) : pick_tile<false>(sg, mn);
+    op->grid = dim3((d->n + 127) / 128, (d->m + mn - 1) / mn, d->splits);
+    const int scale_row = sg * (wide ? 4 : 2), zero_row = sg >= 2 ? sg / 2 : 1;
+    const int stage = (2 * mn * 128 + 8192 + 128 * (scale_row + zero_row) + 1023) / 1024 * 1024;
+    p.wide = wide; p.stage_bytes = static_cast<uint32_t>(stage);
+    p.stages = std::min(kMaxInt4Stages, (227 * 1024 - 1024 - 1024 - 2 * 32768) / stage);
+    op->smem = 2 * 32768 + p.stages * stage + 1024;
+    EncodeTiledFn enc = get_encode_tiled();
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(d->k), static_cast<cuuint64_t>(d->m)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.x_ld) * 2};
+    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(mn)}, ones[2] = {1, 1};
+    if (enc == nullptr ||
+        enc(&op->tm_x, d->dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+            const_cast<uint8_t*>(p.x), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+      delete op; return fail("tensor map encoding failed");
+    }
+    if (cudaFuncSetAttribute(reinterpret_cast<const void*>(op->tile), cudaFuncAttributeMaxDynamicSharedMemorySize, op->smem) != cudaSuccess) {
+      cudaGetLastError(); delete op; return fail("cannot raise the dynamic shared memory limit");
+    }
   }
+  if (op->grid.y > 65535) { delete op; return fail("too many rows"); }
   return op;
 }

@@ -68,6 +68,27 @@ class NativeOp:
             pass
 
 
+class DeviceOp(NativeOp):
+    """A native op that runs on the device of its tensors, whichever device is current: ``create`` is called with that
+    device current, and a launch without a stream goes to that device's current stream."""
+
+    def __init__(self, create, keep: List[Any], name: str, device: torch.device):
+        with torch.cuda.device(device):
+            super().__init__(create(), keep, name)
+        self.device = device
+        self._index = device.index if device.index is not None else torch.cuda.current_device()
+        self._run = _native.kernels().fdb_op_launch
+
+    def launch(self, stream: Optional[int] = None) -> None:
+        # a decoding step is a chain of launches of a few microseconds: the handle of the current stream is read without
+        # building a Stream object around it
+        s = torch._C._cuda_getCurrentRawStream(self._index) if stream is None else stream
+        if self._run(self.handle, s) != 0:
+            raise RuntimeError(f"{self.name}: launch failed: {_native.last_error()}")
+
+    __call__ = launch
+
+
 class StatusWord:
     """Device int that kernels write a non-zero code to instead of trapping or hanging."""
 

@@ -18,7 +18,7 @@ from typing import Optional
 import torch
 
 from .. import _native
-from .base import DT_BF16, DT_F16, NativeOp, StatusWord, current_stream_ptr
+from .base import DT_BF16, DT_F16, DeviceOp, StatusWord
 
 KEY_TILE = 128          # keys per tile of the tensor-core kernel
 
@@ -95,19 +95,10 @@ def _pitch(t: torch.Tensor, dim: int, least: int) -> int:
     return t.stride(dim) if t.shape[dim] > 1 else (least + 7) // 8 * 8
 
 
-class _DecoderOp(NativeOp):
-    """A planned launch on the device of its tensors, whichever device is current."""
-
-    def __init__(self, desc: _DecoderAttnDesc, keep, name: str, device: torch.device):
-        self.device = device
-        with torch.cuda.device(device):
-            super().__init__(_lib().fdb_decoder_attention_create(ctypes.byref(desc)), keep, name)
-        self.create = ("fdb_decoder_attention_create", None, desc)
-
-    def launch(self, stream: Optional[int] = None) -> None:
-        super().launch(current_stream_ptr(self.device) if stream is None else stream)
-
-    __call__ = launch
+def _make(desc: _DecoderAttnDesc, keep, name: str, device: torch.device) -> DeviceOp:
+    op = DeviceOp(lambda: _lib().fdb_decoder_attention_create(ctypes.byref(desc)), keep, name, device)
+    op.create = ("fdb_decoder_attention_create", None, desc)
+    return op
 
 
 class CausalAttention:
@@ -148,7 +139,7 @@ class CausalAttention:
         dd.k_ld, dd.v_ld = _pitch(k, 0, kv_heads * d), _pitch(v, 0, kv_heads * d)
         dd.dtype, dd.n_seq, dd.rows, dd.max_len = _DTYPES[q.dtype], n, rows, min(max_len, rows)
         dd.H, dd.Hk, dd.D, dd.causal, dd.scale = heads, kv_heads, d, int(bool(causal)), scale
-        self.ops = [_DecoderOp(dd, [q, k, v, out, seq_start, seq_len, self.status], "causal_attention", q.device)]
+        self.ops = [_make(dd, [q, k, v, out, seq_start, seq_len, self.status], "causal_attention", q.device)]
 
     def launch(self, stream: Optional[int] = None) -> None:
         for op in self.ops:
@@ -240,8 +231,8 @@ class SharedPrefixAttention:
             dd.k_item, dd.v_item = _pitch(k, 0, 0), _pitch(v, 0, 0)
         dd.dtype, dd.prefix_form, dd.rows, dd.prefix_rows, dd.own_rows = _DTYPES[q.dtype], 1, b, rows, own
         dd.H, dd.Hk, dd.D, dd.splits, dd.own_splits, dd.scale = heads, kv_heads, d, splits, own_splits, scale
-        self.ops = [_DecoderOp(dd, [q, prefix_k, prefix_v, k, v, out, seq_len, prefix_len, self.part_o, self.part_ml,
-                                    self.own_o, self.own_ml, self.counter, self.status], "shared_prefix_attention", dev)]
+        self.ops = [_make(dd, [q, prefix_k, prefix_v, k, v, out, seq_len, prefix_len, self.part_o, self.part_ml,
+                               self.own_o, self.own_ml, self.counter, self.status], "shared_prefix_attention", dev)]
 
     def launch(self, stream: Optional[int] = None) -> None:
         for op in self.ops:

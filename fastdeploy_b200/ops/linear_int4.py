@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native
-from .base import DT_BF16, DT_F16, DT_F32, NativeOp, current_stream_ptr
+from .base import DT_BF16, DT_F16, DT_F32, DeviceOp, StatusWord, current_stream_ptr
 
 GROUPS = (16, 32, 64, 128, 256)
 _DTYPES = {torch.float16: DT_F16, torch.bfloat16: DT_BF16}
@@ -23,9 +23,10 @@ _SCALE_DTYPES = {torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.float32: 
 
 
 class _Int4Desc(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "y", "bias", "w", "scales", "zeros", "x_pad")] + \
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "y", "bias", "w", "scales", "zeros", "x_pad", "status", "partial",
+                                             "counter")] + \
                [("x_ld", ctypes.c_longlong), ("y_ld", ctypes.c_longlong)] + \
-               [(n, ctypes.c_int) for n in ("dtype", "scale_dtype", "m", "n", "k", "group")]
+               [(n, ctypes.c_int) for n in ("dtype", "scale_dtype", "m", "n", "k", "group", "tile_rows", "splits")]
 
 
 def _lib():
@@ -129,12 +130,24 @@ def pack_linear_weight_int4(qweight: torch.Tensor, scales: torch.Tensor, zero_po
     return Int4Weight(data, out_s, out_z, n, k, group)
 
 
-class Int4Linear(NativeOp):
+VECTOR_ROWS = 8
+
+
+def _tile_form(m: int, weight: Int4Weight, sms: int) -> Tuple[int, int]:
+    """(rows of x per tile, splits of K) of the tensor-core kernel, (0, 1) for the vector kernel."""
+    if m <= VECTOR_ROWS:
+        return 0, 1
+    rows = 16 if m <= 16 else 32 if m <= 32 else 64
+    ctas, k_tiles = -(-weight.n // 128) * -(-m // rows), -(-weight.k // 128)
+    return rows, max(1, min(sms // ctas, k_tiles // 4))
+
+
+class Int4Linear(DeviceOp):
     """Planned ``y[M, n] = x[M, k] @ W^T + bias`` over fixed buffers: ``x`` and ``y`` fp16 or bf16 with any row pitch,
     ``bias`` fp32 ``[n]``."""
 
     def __init__(self, x: torch.Tensor, weight: Int4Weight, y: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
-                 name: str = "int4_linear"):
+                 status: Optional[StatusWord] = None, name: str = "int4_linear"):
         if x.dim() != 2 or y.dim() != 2 or x.shape[0] != y.shape[0] or x.shape[0] < 1:
             raise ValueError(f"x [M, {weight.k}] and y [M, {weight.n}] are needed, got {tuple(x.shape)} and {tuple(y.shape)}")
         if x.shape[1] != weight.k or y.shape[1] != weight.n:
@@ -152,26 +165,28 @@ class Int4Linear(NativeOp):
         for what, t in (("x", x), ("y", y), ("bias", bias)):
             if t is not None and t.device != weight.data.device:
                 raise ValueError(f"{what} is on {t.device}, the weight on {weight.data.device}")
-        self.device = x.device
         d = _Int4Desc()
         d.x_ld, d.y_ld = (x.stride(0), y.stride(0)) if m > 1 else (-(-weight.k // 8) * 8, weight.n)
         aligned = x.data_ptr() % 16 == 0 and d.x_ld % 8 == 0 and weight.k % 8 == 0
         # rows that 16-byte loads cannot take are copied to aligned ones first
         self.x_pad = None if aligned else torch.zeros(m, -(-weight.k // 8) * 8, dtype=x.dtype, device=x.device)
-        d.x, d.y, d.w, d.scales = x.data_ptr(), y.data_ptr(), weight.data.data_ptr(), weight.scales.data_ptr()
-        for field, t in (("bias", bias), ("zeros", weight.zeros), ("x_pad", self.x_pad)):
+        # the kernel reads scales of x's type or fp32; the other 16-bit type is widened, which changes no value
+        scales = weight.scales if weight.scales.dtype in (x.dtype, torch.float32) else weight.scales.float()
+        d.x, d.y, d.w, d.scales = x.data_ptr(), y.data_ptr(), weight.data.data_ptr(), scales.data_ptr()
+        self.status = status or StatusWord(x.device)
+        tile_rows, splits = _tile_form(m, weight, torch.cuda.get_device_properties(x.device).multi_processor_count)
+        columns = -(-weight.n // 128) * -(-m // max(1, tile_rows))
+        self.partial = torch.empty(splits, m, weight.n, dtype=torch.float32, device=x.device) if splits > 1 else None
+        self.counter = torch.zeros(columns, dtype=torch.int32, device=x.device) if splits > 1 else None
+        d.tile_rows, d.splits, d.status = tile_rows, splits, self.status.ptr
+        for field, t in (("bias", bias), ("zeros", weight.zeros), ("x_pad", self.x_pad), ("partial", self.partial),
+                         ("counter", self.counter)):
             setattr(d, field, t.data_ptr() if t is not None else None)
-        d.dtype, d.scale_dtype = _DTYPES[x.dtype], _SCALE_DTYPES[weight.scales.dtype]
+        d.dtype, d.scale_dtype = _DTYPES[x.dtype], _SCALE_DTYPES[scales.dtype]
         d.m, d.n, d.k, d.group = m, weight.n, weight.k, weight.group
-        with torch.cuda.device(self.device):
-            super().__init__(_lib().fdb_int4_linear_create(ctypes.byref(d)),
-                             [x, y, bias, weight.data, weight.scales, weight.zeros, self.x_pad], name)
+        super().__init__(lambda: _lib().fdb_int4_linear_create(ctypes.byref(d)),
+                         [x, y, bias, weight.data, scales, weight.zeros, self.x_pad, self.partial, self.counter, self.status], name, x.device)
         self.create = ("fdb_int4_linear_create", None, d)
-
-    def launch(self, stream: Optional[int] = None) -> None:
-        super().launch(current_stream_ptr(self.device) if stream is None else stream)
-
-    __call__ = launch
 
 
 def linear_int4(x: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
