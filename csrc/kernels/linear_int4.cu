@@ -22,46 +22,47 @@ namespace fdb {
 // Descriptor shared with ops/linear_int4.py.
 struct Int4Desc {
   const void* x; void* y; const float* bias;
-  const void* w; const void* scales; const void* zeros;     // packed by fdb_int4_pack; zeros may be null (8 everywhere)
+  const void* w;                                            // packed by fdb_int4_pack
   void* x_pad;                                              // [m][k rounded up to 8] when x's rows are not 16-byte aligned
   int* status;
-  float* partial; unsigned* counter;                        // tile form with splits: [splits][m][n], one per CTA column
   long long x_ld, y_ld;
-  int dtype, scale_dtype, m, n, k, group, tile_rows, splits;  // tile_rows: 0 = the vector kernel, else x rows per tile
+  int dtype, scale_dtype, has_zeros, m, n, k, group, tile_rows, splits;   // tile_rows: 0 = the vector kernel, else x rows per tile
 };
 
 struct Int4Params {
   const uint8_t* x; uint8_t* y; const float* bias;
-  const uint4* w; const uint8_t* scales; const uint8_t* zeros;
-  int* status; float* partial; unsigned* counter;
+  const uint8_t* w;
+  int* status;
   long long x_ld, y_ld;
-  int m, n, k, k_tiles, splits, stages, wide;
-  uint32_t stage_bytes;
+  int m, n, k, k_tiles, splits, stages, wide, has_zeros;
+  uint32_t stage_bytes, block_bytes;      // of a ring stage and of a packed block
 };
 
 // ---------------------------------------------------------------------------------------------------------- packing
-// Source: rows of nibbles, the even element in the low half of a byte, groups padded to whole ones. Packed weights: for
-// each tile of 16 rows x 128 of K, 2 x 32 x 16 bytes: half h and lane (g, t) hold row g + 8 h; word j its elements of
-// K block j * 32; nibble i / 2 + 4 (i % 2) of the word is element i of the lane: k = 8 t + i, or, for groups of 16,
-// 4 t + i of the first group and of the second one. Scales: [tile][16 rows][128 / min(g, 128)], zero points alike in
-// nibbles. What lies behind N or K is q = z with scale 0.
+// Source: rows of nibbles, the even element in the low half of a byte, groups padded to whole ones. Packed: one block
+// for each 128 rows x 128 of K, K innermost, with all that a product needs of them (one copy brings it on chip): the
+// weights of eight tiles of 16 rows, the scales [128 rows][128 / min(g, 128)], and, unless all are 8, the zero points
+// alike, two to a byte. A tile has 1024 bytes: row r has 64 of them, in four pieces of 16; piece t lies at place
+// (t + r / 2) % 4, so that eight consecutive rows' pieces t meet different banks. Word j of a piece holds eight elements
+// of K block j * 32; nibble i / 2 + 4 (i % 2) of the word is element i: k = 8 t + i, or, for groups of 16, 4 t + i of the
+// first group (i < 4) and 4 t + i - 4 of the second. What lies behind N or K is q = z with scale 0.
 __device__ __forceinline__ int nibble_zero(const uint8_t* zeros, long long row, int blk, int zero_bytes) {
   if (zeros == nullptr) return 8;
   const int b = zeros[row * zero_bytes + (blk >> 1)];
   return (blk & 1) ? b >> 4 : b & 15;
 }
 
-__global__ void int4_pack_weights(const uint8_t* __restrict__ q, const uint8_t* __restrict__ zeros, uint32_t* __restrict__ out,
-                                  int n, int k, int group, int k_tiles, long long words) {
+__global__ void int4_pack_weights(const uint8_t* __restrict__ q, const uint8_t* __restrict__ zeros, uint8_t* __restrict__ out,
+                                  int n, int k, int group, int k_tiles, long long block_bytes, long long words) {
   const int blocks = (k + group - 1) / group, zero_bytes = (blocks + 1) / 2;
   const long long row_bytes = static_cast<long long>(blocks) * group / 2;
   for (long long w = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; w < words;
        w += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const int j = static_cast<int>(w & 3), lane = static_cast<int>(w >> 2) & 31, half = static_cast<int>(w >> 7) & 1;
-    const long long tile = w >> 8;
-    const int kt = static_cast<int>(tile % k_tiles);
-    const long long row = tile / k_tiles * 16 + (lane >> 2) + 8 * half;
-    const int t = lane & 3;
+    const int j = static_cast<int>(w & 3), place = static_cast<int>(w >> 2) & 3, r = static_cast<int>(w >> 4) & 127;
+    const long long block = w >> 11;
+    const int kt = static_cast<int>(block % k_tiles);
+    const long long row = block / k_tiles * 128 + r;
+    const int t = (place - (r >> 1)) & 3;
     uint32_t v = 0;
     for (int i = 0; i < 8; ++i) {
       const int in = group == 16 ? (i >> 2) * 16 + 4 * t + (i & 3) : 8 * t + i;
@@ -77,30 +78,32 @@ __global__ void int4_pack_weights(const uint8_t* __restrict__ q, const uint8_t* 
       }
       v |= e << (4 * (i >> 1) + 16 * (i & 1));
     }
-    out[w] = v;
+    *reinterpret_cast<uint32_t*>(out + block * block_bytes + (w & 2047) * 4) = v;
   }
 }
 
-// One thread per (tile, row): the scales of the tile's groups and their zero points.
+// One thread per row of a block: the scales of its groups and their zero points.
 template <typename S>
-__global__ void int4_pack_scales(const S* __restrict__ s, const uint8_t* __restrict__ zeros, S* __restrict__ out,
-                                 uint8_t* __restrict__ out_zeros, int n, int k, int group, int k_tiles, long long count) {
+__global__ void int4_pack_scales(const S* __restrict__ s, const uint8_t* __restrict__ zeros, uint8_t* __restrict__ out, int n,
+                                 int k, int group, int k_tiles, long long block_bytes, long long count) {
   const int blocks = (k + group - 1) / group, zero_bytes = (blocks + 1) / 2;
   const int per = 128 / min(group, 128);
   for (long long x = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; x < count;
        x += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const long long tile = x >> 4, row = tile / k_tiles * 16 + (x & 15);
-    const int kt = static_cast<int>(tile % k_tiles);
+    const long long block = x >> 7, row = block / k_tiles * 128 + (x & 127);
+    const int kt = static_cast<int>(block % k_tiles);
+    uint8_t* to = out + block * block_bytes + 8192;
     uint32_t z = 0;
     for (int i = 0; i < per; ++i) {
       const int blk = static_cast<int>((kt * 128LL + i * (128 / per)) / group);
       const bool in = row < n && blk < blocks;
-      out[x * per + i] = in ? s[row * blocks + blk] : S(0.f);
+      reinterpret_cast<S*>(to)[(x & 127) * per + i] = in ? s[row * blocks + blk] : S(0.f);
       z |= static_cast<uint32_t>(in ? nibble_zero(zeros, row, blk, zero_bytes) : 8) << (4 * i);
     }
-    if (out_zeros != nullptr) {
+    if (zeros != nullptr) {
       const int bytes = max(1, per / 2);
-      for (int i = 0; i < bytes; ++i) out_zeros[x * bytes + i] = static_cast<uint8_t>(z >> (8 * i));
+      uint8_t* zr = to + 128 * per * sizeof(S) + (x & 127) * bytes;
+      for (int i = 0; i < bytes; ++i) zr[i] = static_cast<uint8_t>(z >> (8 * i));
     }
   }
 }
@@ -113,12 +116,6 @@ __global__ void int4_pad_rows(const uint16_t* __restrict__ x, uint16_t* __restri
 }
 
 // ---------------------------------------------------------------------------------------------------------- product
-__device__ __forceinline__ uint4 ld_stream(const uint4* p) {
-  uint4 v;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-
 template <bool BF16>
 __device__ __forceinline__ void int4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -170,19 +167,19 @@ __device__ __forceinline__ void unpack_word(uint32_t w, const ZeroPair& z, uint3
   }
 }
 
-// SG scales of one row of a tile: fp32, or 16-bit of x's type.
+// SG scales of one row of a tile, in shared memory: fp32, or 16-bit of x's type.
 template <bool BF16, bool WIDE, int SG>
 struct ScaleRow {
   uint32_t w[WIDE ? SG : (SG + 1) / 2];
   __device__ __forceinline__ void load(const uint8_t* a) {
     if (WIDE) {
 #pragma unroll
-      for (int i = 0; i < SG; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(a) + i);
+      for (int i = 0; i < SG; ++i) w[i] = reinterpret_cast<const uint32_t*>(a)[i];
     } else if (SG == 1) {
-      w[0] = __ldg(reinterpret_cast<const uint16_t*>(a));
+      w[0] = *reinterpret_cast<const uint16_t*>(a);
     } else {
 #pragma unroll
-      for (int i = 0; i < SG / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(a) + i);
+      for (int i = 0; i < SG / 2; ++i) w[i] = reinterpret_cast<const uint32_t*>(a)[i];
     }
   }
   __device__ __forceinline__ float at(int i) const {
@@ -194,117 +191,127 @@ struct ScaleRow {
 
 template <int SG>
 __device__ __forceinline__ uint32_t load_zeros(const uint8_t* a) {
-  if (SG == 8) return __ldg(reinterpret_cast<const uint32_t*>(a));
-  if (SG == 4) return __ldg(reinterpret_cast<const uint16_t*>(a));
-  return __ldg(a);
+  if (SG == 8) return *reinterpret_cast<const uint32_t*>(a);
+  if (SG == 4) return *reinterpret_cast<const uint16_t*>(a);
+  return *a;
 }
 
 constexpr int kInt4Warps = 8;
 
-// Up to 8 MT rows of x; the CTA's eight warps share 16 weight rows.
+// Up to 8 MT rows of x; the CTA's eight warps share 16 weight rows, each warp a run of tiles along K, which it brings into
+// a ring of its own in shared memory by cp.async (no registers held, nothing to wait for but its own copies).
+constexpr int kVecStages = 4;
+
 template <bool BF16, bool WIDE, bool ZERO, int SG, int MT>
 __global__ void __launch_bounds__(kInt4Warps * 32)
 int4_linear_kernel(const Int4Params p) {
-  __shared__ float red[kInt4Warps * 8 * MT * 16];
-  constexpr int kScaleBytes = 16 * SG * (WIDE ? 4 : 2), kZeroBytes = 16 * (SG >= 2 ? SG / 2 : 1);   // of a tile
+  constexpr uint32_t kScaleRow = SG * (WIDE ? 4 : 2), kZeroRow = SG >= 2 ? SG / 2 : 1;          // bytes of a row of a tile
+  constexpr uint32_t kStage = 1024 + 16 * (kScaleRow + (ZERO ? kZeroRow : 0));
+  extern __shared__ __align__(16) uint8_t ring_raw[];                // [warps][stages][kStage], then the warps' sums
+  float* red = reinterpret_cast<float*>(ring_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int m0 = blockIdx.y * (8 * MT);
   float acc[MT][4] = {};
-  const long long tile0 = static_cast<long long>(blockIdx.x) * p.k_tiles + warp;
-  const uint4* wp = p.w + tile0 * 64 + lane;
-  const uint8_t* sp = p.scales + tile0 * kScaleBytes + g * (kScaleBytes / 16);
-  const uint8_t* zp = ZERO ? p.zeros + tile0 * kZeroBytes + g * (kZeroBytes / 16) : nullptr;
+  const int kt0 = p.k_tiles * warp / kInt4Warps, count = p.k_tiles * (warp + 1) / kInt4Warps - kt0;
+  const int in_block = blockIdx.x & 7;                               // which 16 rows of a block
+  const uint8_t* ring = ring_raw + warp * (kVecStages * kStage);
+  const uint32_t ring_at = smem_u32(ring);
+  const uint8_t* wp = p.w + (static_cast<long long>(blockIdx.x >> 3) * p.k_tiles + kt0) * p.block_bytes + lane * 16;
+  const uint32_t scales_at = 8192 + in_block * (16 * kScaleRow), zeros_at = 8192 + 128 * kScaleRow + in_block * (16 * kZeroRow);
+  auto fetch = [&](int i) {                                          // tile i of the warp; a group of copies either way
+    if (i < count) {
+      const uint32_t at = ring_at + static_cast<uint32_t>(i % kVecStages) * kStage + lane * 16;
+      const uint8_t* block = wp + static_cast<long long>(i) * p.block_bytes;
+      cp_async_16(at, block + in_block * 1024, 16);
+      cp_async_16(at + 512, block + in_block * 1024 + 512, 16);
+      if (lane * 16 < 16 * kScaleRow) cp_async_16(at + 1024, block + scales_at, 16);
+      if (ZERO && lane * 16 < 16 * kZeroRow) cp_async_16(at + 1024 + 16 * kScaleRow, block + zeros_at, 16);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kVecStages - 1; ++i) fetch(i);
+
   const uint8_t* xp[MT];
   bool row_in[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     row_in[i] = m0 + i * 8 + g < p.m;
-    xp[i] = p.x + (row_in[i] ? (m0 + i * 8 + g) * p.x_ld * 2 : 0) + (warp * 128 + (SG == 8 ? 4 : 8) * t) * 2;
+    xp[i] = p.x + (row_in[i] ? (m0 + i * 8 + g) * p.x_ld * 2 : 0) + (kt0 * 128 + (SG == 8 ? 4 : 8) * t) * 2;
   }
-  // Elements of x from this lane's first one to the end of the row, less those that lie ahead: a load is made when it
-  // starts inside the row (K is a multiple of 8 here, so it ends inside too).
-  int left = p.k - warp * 128 - (SG == 8 ? 4 : 8) * t;
-  // The loads of U tiles along K are in flight before the first of them is used.
-  constexpr int U = MT == 1 ? 4 : 2;
-  int todo = (p.k_tiles - warp + kInt4Warps - 1) / kInt4Warps;        // tiles of this warp
-  while (todo > 0) {
-    uint4 w[U][2];
-    ScaleRow<BF16, WIDE, SG> s[U][2];
-    uint32_t z[U][2];
+  // Elements of x from this lane's first one to the end of the row: a load is made when it starts inside the row (K is a
+  // multiple of 8 here, so it ends inside too).
+  int left = p.k - kt0 * 128 - (SG == 8 ? 4 : 8) * t;
+  const uint32_t piece_a = g * 64 + ((t + (g >> 1)) & 3) * 16;       // rows g and g + 8: the same place, 512 bytes apart
+  for (int i = 0; i < count; ++i, left -= 128) {
+    uint4 xb[4][MT];
 #pragma unroll
-    for (int v = 0; v < U; ++v) {
-      if (v < todo) {
-        w[v][0] = ld_stream(wp + v * kInt4Warps * 64);
-        w[v][1] = ld_stream(wp + v * kInt4Warps * 64 + 32);
-        s[v][0].load(sp + v * kInt4Warps * kScaleBytes);
-        s[v][1].load(sp + v * kInt4Warps * kScaleBytes + kScaleBytes / 2);
-        if (ZERO) {
-          z[v][0] = load_zeros<SG>(zp + v * kInt4Warps * kZeroBytes);
-          z[v][1] = load_zeros<SG>(zp + v * kInt4Warps * kZeroBytes + kZeroBytes / 2);
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < MT; ++r) {
+        xb[j][r] = make_uint4(0, 0, 0, 0);
+        const uint8_t* a = xp[r] + j * 64;
+        if (SG == 8) {
+          // groups of 16: the lane's elements are 4 t .. of either group
+          if (row_in[r] && j * 32 < left) { const uint2 h = __ldg(reinterpret_cast<const uint2*>(a)); xb[j][r].x = h.x; xb[j][r].y = h.y; }
+          if (row_in[r] && j * 32 + 16 < left) { const uint2 h = __ldg(reinterpret_cast<const uint2*>(a + 32)); xb[j][r].z = h.x; xb[j][r].w = h.y; }
+        } else if (row_in[r] && j * 32 < left) {
+          xb[j][r] = __ldg(reinterpret_cast<const uint4*>(a));
         }
       }
+#pragma unroll
+    for (int r = 0; r < MT; ++r) xp[r] += 256;
+    cp_async_wait<kVecStages - 2>();
+    __syncwarp();                                                    // every lane's copies of tile i have landed
+    fetch(i + kVecStages - 1);                                       // into the stage that tile i - 1 left
+    const uint8_t* at = ring + (i % kVecStages) * kStage;
+    const uint4 va = *reinterpret_cast<const uint4*>(at + piece_a), vb = *reinterpret_cast<const uint4*>(at + piece_a + 512);
+    ScaleRow<BF16, WIDE, SG> s[2];
+    s[0].load(at + 1024 + g * kScaleRow);
+    s[1].load(at + 1024 + (g + 8) * kScaleRow);
+    uint32_t z[2] = {0x88888888u, 0x88888888u};
+    if (ZERO) {
+      z[0] = load_zeros<SG>(at + 1024 + 16 * kScaleRow + g * kZeroRow);
+      z[1] = load_zeros<SG>(at + 1024 + 16 * kScaleRow + (g + 8) * kZeroRow);
     }
+    float part[MT][4];
 #pragma unroll
-    for (int v = 0; v < U; ++v) {
-      if (v >= todo) break;
-      float part[MT][4];
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t wa = j == 0 ? va.x : j == 1 ? va.y : j == 2 ? va.z : va.w;
+      const uint32_t wb = j == 0 ? vb.x : j == 1 ? vb.y : j == 2 ? vb.z : vb.w;
+      uint32_t ra[4], rb[4];
+      const int g0 = j * 2 * SG / 8;
+      unpack_word<BF16>(wa, zero_pair<BF16>(ZERO ? (z[0] >> (4 * g0)) & 15u : 8u), ra);
+      unpack_word<BF16>(wb, zero_pair<BF16>(ZERO ? (z[1] >> (4 * g0)) & 15u : 8u), rb);
+      if (SG == 8 && ZERO) {                            // the word's second half belongs to the next group
+        uint32_t other[4];
+        unpack_word<BF16>(wa, zero_pair<BF16>((z[0] >> (4 * g0 + 4)) & 15u), other);
+        ra[2] = other[2]; ra[3] = other[3];
+        unpack_word<BF16>(wb, zero_pair<BF16>((z[1] >> (4 * g0 + 4)) & 15u), other);
+        rb[2] = other[2]; rb[3] = other[3];
+      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint4 xb[MT];
+      for (int u = 0; u < 2; ++u) {                     // the two K = 16 steps of a K block of 32
+        const int grp = (j * 2 + u) * SG / 8;
+        const bool first = SG == 8 || (j * 2 + u) % (8 / SG) == 0, last = SG == 8 || (j * 2 + u + 1) % (8 / SG) == 0;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          xb[i] = make_uint4(0, 0, 0, 0);
-          const uint8_t* a = xp[i] + (v * kInt4Warps * 128 + j * 32) * 2;
-          const int ahead = v * kInt4Warps * 128 + j * 32;
-          if (SG == 8) {
-            // groups of 16: the lane's elements are 4 t .. of either group
-            if (row_in[i] && ahead < left) { const uint2 h = __ldg(reinterpret_cast<const uint2*>(a)); xb[i].x = h.x; xb[i].y = h.y; }
-            if (row_in[i] && ahead + 16 < left) { const uint2 h = __ldg(reinterpret_cast<const uint2*>(a + 32)); xb[i].z = h.x; xb[i].w = h.y; }
-          } else if (row_in[i] && ahead < left) {
-            xb[i] = __ldg(reinterpret_cast<const uint4*>(a));
-          }
-        }
-        const uint32_t wa = j == 0 ? w[v][0].x : j == 1 ? w[v][0].y : j == 2 ? w[v][0].z : w[v][0].w;
-        const uint32_t wb = j == 0 ? w[v][1].x : j == 1 ? w[v][1].y : j == 2 ? w[v][1].z : w[v][1].w;
-        uint32_t ra[4], rb[4];
-        const int g0 = j * 2 * SG / 8;
-        unpack_word<BF16>(wa, zero_pair<BF16>(ZERO ? (z[v][0] >> (4 * g0)) & 15u : 8u), ra);
-        unpack_word<BF16>(wb, zero_pair<BF16>(ZERO ? (z[v][1] >> (4 * g0)) & 15u : 8u), rb);
-        if (SG == 8 && ZERO) {                            // the word's second half belongs to the next group
-          uint32_t other[4];
-          unpack_word<BF16>(wa, zero_pair<BF16>((z[v][0] >> (4 * g0 + 4)) & 15u), other);
-          ra[2] = other[2]; ra[3] = other[3];
-          unpack_word<BF16>(wb, zero_pair<BF16>((z[v][1] >> (4 * g0 + 4)) & 15u), other);
-          rb[2] = other[2]; rb[3] = other[3];
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {                     // the two K = 16 steps of a K block of 32
-          const int grp = (j * 2 + u) * SG / 8;
-          const bool first = SG == 8 || (j * 2 + u) % (8 / SG) == 0, last = SG == 8 || (j * 2 + u + 1) % (8 / SG) == 0;
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            if (first) part[i][0] = part[i][1] = part[i][2] = part[i][3] = 0.f;
-            int4_mma<BF16>(part[i], ra[2 * u], rb[2 * u], ra[2 * u + 1], rb[2 * u + 1], u == 0 ? xb[i].x : xb[i].z,
-                           u == 0 ? xb[i].y : xb[i].w);
-            if (last) {
-              const float s0 = s[v][0].at(grp), s1 = s[v][1].at(grp);
-              acc[i][0] = fmaf(part[i][0], s0, acc[i][0]);
-              acc[i][1] = fmaf(part[i][1], s0, acc[i][1]);
-              acc[i][2] = fmaf(part[i][2], s1, acc[i][2]);
-              acc[i][3] = fmaf(part[i][3], s1, acc[i][3]);
-            }
+        for (int r = 0; r < MT; ++r) {
+          if (first) part[r][0] = part[r][1] = part[r][2] = part[r][3] = 0.f;
+          int4_mma<BF16>(part[r], ra[2 * u], rb[2 * u], ra[2 * u + 1], rb[2 * u + 1], u == 0 ? xb[j][r].x : xb[j][r].z,
+                         u == 0 ? xb[j][r].y : xb[j][r].w);
+          if (last) {
+            const float s0 = s[0].at(grp), s1 = s[1].at(grp);
+            acc[r][0] = fmaf(part[r][0], s0, acc[r][0]);
+            acc[r][1] = fmaf(part[r][1], s0, acc[r][1]);
+            acc[r][2] = fmaf(part[r][2], s1, acc[r][2]);
+            acc[r][3] = fmaf(part[r][3], s1, acc[r][3]);
           }
         }
       }
     }
-    todo -= U;
-    left -= U * kInt4Warps * 128;
-    wp += U * kInt4Warps * 64;
-    sp += U * kInt4Warps * kScaleBytes;
-    if (ZERO) zp += U * kInt4Warps * kZeroBytes;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) xp[i] += U * kInt4Warps * 256;
   }
+  cp_async_wait<0>();
+  __syncthreads();                                                   // the rings become the warps' sums
   constexpr int kCols = 8 * MT;
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -328,13 +335,17 @@ int4_linear_kernel(const Int4Params p) {
 // ------------------------------------------------------------------------------------------------ more rows: tcgen05
 // From a few rows on, mma.sync (measured: 550 TFLOP/s) and the reads of x by every 16 weight rows cost more than the
 // weights' bytes. Here a CTA takes 128 weight rows as the M side of tcgen05.mma and MN rows of x as its N side:
-//   producer    bulk copies of the packed tile [128 x 128 of K] with its scales and zero points, TMA for x
-//   dequant     eight warps turn the tile into q - z in 16 bits (exact), K-major and 128B-swizzled in shared memory
+//   producer    one bulk copy of the packed block [128 x 128 of K] with its scales and zero points, TMA for x
+//   dequant     two groups of four warps take turns: q - z in 16 bits (exact), a weight row per thread, straight into
+//               tensor memory as the A operand (through shared memory it would be written and read back once per MMA:
+//               112 KB a tile in all, 900 clocks of the 128 bytes a clock; that form measured 80 us where this one's
+//               figure is in the table of the design notes' operator section)
 //   MMA         one product per scale group into one of four accumulators in tensor memory
 //   drain       four warps, a weight row per thread: sum += scale * accumulator, in fp32
-// so that the scales meet fp32 sums here too and the two kernels differ only in the order of their additions.
+// so that the scales meet fp32 sums here too and the two kernels differ only in the order of their additions. Few weight
+// rows: up to eight CTAs of a cluster split K and add their sums, in their order, over distributed shared memory.
 constexpr int kTileThreads = 512;
-constexpr int kDequantWarps = 8;
+constexpr int kDequantGroups = 2;
 constexpr int kMaxInt4Stages = 8;
 
 template <bool BF16, int SG, int MN>
@@ -344,16 +355,16 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
   __shared__ __align__(8) uint64_t bars[2 * kMaxInt4Stages + 12];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
-  __shared__ unsigned ticket;
   volatile int* abort_flag = &abort_word;
   constexpr uint32_t kX = 2 * MN * 128, kW = 8192;
   constexpr uint32_t kZeroRow = SG >= 2 ? SG / 2 : 1;
-  const bool has_zeros = p.zeros != nullptr;
+  const bool has_zeros = p.has_zeros != 0;
   const uint32_t scale_row = SG * (p.wide ? 4 : 2), stage_bytes = p.stage_bytes;
-  constexpr uint32_t kTmemCols = 4 * MN < 32 ? 32 : 4 * MN;
+  constexpr uint32_t kA = 4 * MN;                                   // tensor memory: four accumulators, then A
+  constexpr uint32_t kTmemCols = kA + kDequantGroups * 64 <= 256 ? 256 : 512;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t s_a = base, s_ring = base + 2 * 32768;
+  const uint32_t s_ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint8_t* ring = smem_raw + (s_ring - smem_u32(smem_raw));
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   auto full = [&](int i) { return bar(i); };
   auto empty = [&](int i) { return bar(kMaxInt4Stages + i); };
@@ -364,13 +375,12 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
   const int kt0 = static_cast<int>(static_cast<long long>(p.k_tiles) * blockIdx.z / p.splits);
   const int kt1 = static_cast<int>(static_cast<long long>(p.k_tiles) * (blockIdx.z + 1) / p.splits);
   const int n_it = kt1 - kt0;
-  const int row_tiles = (p.n + 15) / 16, rt0 = blockIdx.x * 8, rts = min(8, row_tiles - rt0);
   const int m0 = blockIdx.y * MN;
 
   if (tid == 0) {
     abort_word = 0;
-    for (int i = 0; i < kMaxInt4Stages; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), kDequantWarps + 1 + 4); }
-    for (int i = 0; i < 2; ++i) { mbar_init(a_full(i), kDequantWarps); mbar_init(a_empty(i), 1); }
+    for (int i = 0; i < kMaxInt4Stages; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 4 + 1 + 4); }
+    for (int i = 0; i < kDequantGroups; ++i) { mbar_init(a_full(i), 4); mbar_init(a_empty(i), 1); }
     for (int i = 0; i < 4; ++i) { mbar_init(d_full(i), 1); mbar_init(d_empty(i), 4); }
     fence_mbar_init();
     prefetch_tensormap(&tm_x);
@@ -383,6 +393,11 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  float acc[MN];                                                    // of the drain warps
+#pragma unroll
+  for (int i = 0; i < MN; ++i) acc[i] = 0.f;
+  const int row = (warp & 3) * 32 + lane;                           // the weight row of a drain or dequant thread
+  const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
 
   if (warp == 0) {
     // ------------------------------------------------------------------------------------------------- producer
@@ -393,20 +408,10 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
       if (round > 0) ok = mbar_wait_warp(empty(st), (round - 1) & 1, abort_flag, kStatusTimeoutProducer);
       if (!ok) break;
       const uint32_t at = s_ring + static_cast<uint32_t>(st) * stage_bytes;
-      const uint32_t bytes = kX + static_cast<uint32_t>(rts) * (1024 + 16 * (scale_row + (has_zeros ? kZeroRow : 0)));
-      if (lane == 0) mbar_arrive_expect_tx(full(st), bytes);
-      __syncwarp();
-      const int r = lane & 7;
-      const long long tile = static_cast<long long>(rt0 + r) * p.k_tiles + kt0 + it;
-      if (lane < 8) {
-        if (r < rts) bulk_load(at + kX + r * 1024, p.w + tile * 64, 1024, full(st));
-      } else if (lane < 16) {
-        if (r < rts) bulk_load(at + kX + kW + r * 16 * scale_row, p.scales + tile * (16 * scale_row), 16 * scale_row, full(st));
-      } else if (lane < 24) {
-        if (has_zeros && r < rts)
-          bulk_load(at + kX + kW + 128 * scale_row + r * 16 * kZeroRow, p.zeros + tile * (16 * kZeroRow), 16 * kZeroRow, full(st));
-      } else if (lane < 26) {
-        tma_load_2d(at + (lane - 24) * (MN * 128), &tm_x, full(st), (kt0 + it) * 128 + (lane - 24) * 64, m0);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(full(st), kX + p.block_bytes);
+        bulk_load(at + kX, p.w + (static_cast<long long>(blockIdx.x) * p.k_tiles + kt0 + it) * p.block_bytes, p.block_bytes, full(st));
+        for (int c = 0; c < 2; ++c) tma_load_2d(at + c * (MN * 128), &tm_x, full(st), (kt0 + it) * 128 + c * 64, m0);
       }
       issued = it + 1;
     }
@@ -423,10 +428,10 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
       const uint32_t idesc = make_idesc(BF16 ? 1u : 0u, 128, MN);
       bool ok = true;
       for (int it = 0; ok && it < n_it; ++it) {
-        const int st = it % p.stages, buf = it & 1;
+        const int st = it % p.stages, buf = it % kDequantGroups;
         ok = mbar_wait(full(st), (it / p.stages) & 1, abort_flag, kStatusTimeoutMma) &&
-             mbar_wait(a_full(buf), (it >> 1) & 1, abort_flag, kStatusTimeoutMma);
-        const uint64_t ad = make_kmajor_desc(s_a + buf * 32768, 128);
+             mbar_wait(a_full(buf), (it / kDequantGroups) & 1, abort_flag, kStatusTimeoutMma);
+        const uint32_t ta = tmem + kA + buf * 64;
         const uint64_t bd = make_kmajor_desc(s_ring + static_cast<uint32_t>(st) * stage_bytes, 128);
         for (int g = 0; ok && g < SG; ++g) {
           const int q = it * SG + g, d = q & 3;
@@ -436,8 +441,8 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
 #pragma unroll
           for (int x = 0; x < 8 / SG; ++x) {
             const int step = g * (8 / SG) + x;
-            umma_f16(tmem + d * MN, ad + (step >> 2) * (16384 >> 4) + (step & 3) * 2,
-                     bd + (step >> 2) * ((MN * 128) >> 4) + (step & 3) * 2, idesc, x != 0 ? 1u : 0u);
+            umma_f16_ts(tmem + d * MN, ta + step * 8, bd + (step >> 2) * ((MN * 128) >> 4) + (step & 3) * 2, idesc,
+                        x != 0 ? 1u : 0u);
           }
           umma_commit(d_full(d));
         }
@@ -450,64 +455,62 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
     __syncwarp();
   } else if (warp >= 8) {
     // -------------------------------------------------------------------------------------------------- dequant
-    const int d = warp - 8, g = lane >> 2, t = lane & 3;
+    const int group = (warp - 8) >> 2, r16 = row & 15;
     bool ok = true;
-    for (int it = 0; ok && it < n_it; ++it) {
-      const int st = it % p.stages, buf = it & 1;
+    for (int it = group; ok && it < n_it; it += kDequantGroups) {
+      const int st = it % p.stages, round = it / kDequantGroups;
       ok = mbar_wait_warp(full(st), (it / p.stages) & 1, abort_flag, kStatusTimeoutProducer);
-      if (ok && it >= 2) ok = mbar_wait_warp(a_empty(buf), ((it >> 1) - 1) & 1, abort_flag, kStatusTimeoutMma);
       if (!ok) break;
-      const uint8_t* stage = smem_raw + (s_ring - smem_u32(smem_raw)) + static_cast<uint32_t>(st) * stage_bytes;
-      const uint32_t to = s_a + buf * 32768;
+      const uint8_t* stage = ring + static_cast<uint32_t>(st) * stage_bytes;
+      uint4 v[4];                                                   // v[t], word j: K elements j * 32 + 8 t ..
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = d * 16 + g + 8 * h;
-        const uint4 v = *reinterpret_cast<const uint4*>(stage + kX + d * 1024 + h * 512 + lane * 16);
-        uint32_t z = 0x88888888u;
-        if (has_zeros) {
-          const uint8_t* zr = stage + kX + kW + 128 * scale_row + row * kZeroRow;
-          z = SG == 8 ? *reinterpret_cast<const uint32_t*>(zr) : SG == 4 ? *reinterpret_cast<const uint16_t*>(zr) : *zr;
-        }
+      for (int t = 0; t < 4; ++t)
+        v[t] = *reinterpret_cast<const uint4*>(stage + kX + (row >> 4) * 1024 + r16 * 64 + ((t + (r16 >> 1)) & 3) * 16);
+      uint32_t z = 0x88888888u;
+      if (has_zeros) z = load_zeros<SG>(stage + kX + kW + 128 * scale_row + row * kZeroRow);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty(st));
+      if (round > 0) ok = mbar_wait_warp(a_empty(group), (round - 1) & 1, abort_flag, kStatusTimeoutMma);
+      if (!ok) break;
+      tc_fence_after();
 #pragma unroll
-        for (int jj = 0; jj < 4; ++jj) {
-          // lanes of odd g take the words of a chunk in the other order: two rows' stores then meet different banks
-          const int j = jj ^ (g & 1), c = jj >> 1;
-          const uint32_t w0 = c == 0 ? v.x : v.z, w1 = c == 0 ? v.y : v.w;
-          const uint32_t word = (j & 1) ? w1 : w0;
-          const uint32_t at = to + c * 16384 + row * 128;
-          uint32_t o[4];
-          if (SG == 8) {
-            uint32_t o2[4];
-            unpack_word<BF16>(word, zero_pair<BF16>((z >> (8 * j)) & 15u), o);
-            unpack_word<BF16>(word, zero_pair<BF16>((z >> (8 * j + 4)) & 15u), o2);
-            const uint32_t unit = (j & 1) * 4 + (t >> 1);
-            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + ((unit ^ g) << 4) + (t & 1) * 8), "r"(o[0]), "r"(o[1]) : "memory");
-            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + (((unit + 2) ^ g) << 4) + (t & 1) * 8), "r"(o2[2]), "r"(o2[3]) : "memory");
-          } else {
-            const int grp = SG == 1 ? 0 : SG == 2 ? c : j;
-            unpack_word<BF16>(word, zero_pair<BF16>((z >> (4 * grp)) & 15u), o);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + ((((j & 1) * 4 + t) ^ g) << 4)), "r"(o[0]),
-                         "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+      for (int half = 0; half < 2; ++half) {                        // 64 of K, 32 columns of tensor memory, at a time
+        uint32_t o[32];
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const int j = half * 2 + jj;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t word = j == 0 ? v[t].x : j == 1 ? v[t].y : j == 2 ? v[t].z : v[t].w;
+            uint32_t e[4];
+            if (SG == 8) {                                          // elements 4 t .. of the two groups of 16
+              uint32_t e2[4];
+              unpack_word<BF16>(word, zero_pair<BF16>((z >> (8 * j)) & 15u), e);
+              unpack_word<BF16>(word, zero_pair<BF16>((z >> (8 * j + 4)) & 15u), e2);
+              o[jj * 16 + 2 * t] = e[0]; o[jj * 16 + 2 * t + 1] = e[1];
+              o[jj * 16 + 8 + 2 * t] = e2[2]; o[jj * 16 + 8 + 2 * t + 1] = e2[3];
+            } else {
+              unpack_word<BF16>(word, zero_pair<BF16>((z >> (4 * (j * SG / 4))) & 15u), e);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o[jj * 16 + 4 * t + x] = e[x];
+            }
           }
         }
+        tmem_st_32x32(tmem + lanes + kA + group * 64 + half * 32, o);
       }
-      fence_proxy_async_smem();
+      tmem_st_wait();
+      tc_fence_before();
       __syncwarp();
-      if (lane == 0) { mbar_arrive(a_full(buf)); mbar_arrive(empty(st)); }
+      if (lane == 0) mbar_arrive(a_full(group));
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------------------------------------------- drain
-    const int row = (warp & 3) * 32 + lane;
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    float acc[MN];
-#pragma unroll
-    for (int i = 0; i < MN; ++i) acc[i] = 0.f;
     bool ok = true;
     for (int it = 0; ok && it < n_it; ++it) {
       const int st = it % p.stages;
       ok = mbar_wait_warp(full(st), (it / p.stages) & 1, abort_flag, kStatusTimeoutProducer);
       if (!ok) break;
-      const uint8_t* sr = smem_raw + (s_ring - smem_u32(smem_raw)) + static_cast<uint32_t>(st) * stage_bytes + kX + kW + row * scale_row;
+      const uint8_t* sr = ring + static_cast<uint32_t>(st) * stage_bytes + kX + kW + row * scale_row;
       float s[SG];
 #pragma unroll
       for (int g = 0; g < SG; ++g) {
@@ -543,8 +546,8 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
         if (lane == 0) mbar_arrive(d_empty(d));
       }
     }
-    const long long n = static_cast<long long>(blockIdx.x) * 128 + row;
-    if (ok && n_it > 0 && p.splits == 1) {
+    if (p.splits == 1 && ok) {
+      const long long n = static_cast<long long>(blockIdx.x) * 128 + row;
       const float b = p.bias != nullptr && n < p.n ? __ldg(p.bias + n) : 0.f;
 #pragma unroll
       for (int i = 0; i < MN; ++i) {
@@ -553,34 +556,30 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
         if (BF16) *reinterpret_cast<__nv_bfloat16*>(y) = __float2bfloat16_rn(acc[i] + b);
         else *reinterpret_cast<__half*>(y) = __float2half_rn(acc[i] + b);
       }
-    } else if (p.splits > 1) {
-      // the last CTA of a column to arrive adds the splits' sums in their order
-#pragma unroll
-      for (int i = 0; i < MN; ++i)
-        if (m0 + i < p.m && n < p.n) __stcg(p.partial + (static_cast<long long>(blockIdx.z) * p.m + m0 + i) * p.n + n, acc[i]);
-      __threadfence();
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      const int column = blockIdx.y * gridDim.x + blockIdx.x;
-      if (warp == 4 && lane == 0) {
-        ticket = atomicAdd(p.counter + column, 1u);
-        if (ticket == static_cast<unsigned>(p.splits) - 1u) p.counter[column] = 0u;       // ready for the next launch
-      }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (ticket == static_cast<unsigned>(p.splits) - 1u && n < p.n) {
-        __threadfence();
-        const float b = p.bias != nullptr ? __ldg(p.bias + n) : 0.f;
-        for (int i = 0; i < MN && m0 + i < p.m; ++i) {
-          float v = 0.f;
-          for (int z = 0; z < p.splits; ++z) v += __ldcg(p.partial + (static_cast<long long>(z) * p.m + m0 + i) * p.n + n);
-          uint8_t* y = p.y + ((m0 + i) * p.y_ld + n) * 2;
-          if (BF16) *reinterpret_cast<__nv_bfloat16*>(y) = __float2bfloat16_rn(v + b);
-          else *reinterpret_cast<__half*>(y) = __float2half_rn(v + b);
-        }
-      }
     }
     tc_fence_before();
   }
-  __syncthreads();
+  __syncthreads();                                                  // every copy and every MMA is done with the ring
+  if (p.splits > 1) {
+    float* sums = reinterpret_cast<float*>(const_cast<uint8_t*>(ring));            // [MN][128] of this CTA's part of K
+    if (warp >= 4 && warp < 8) {
+#pragma unroll
+      for (int i = 0; i < MN; ++i) sums[i * 128 + row] = acc[i];
+    }
+    cluster_sync_all();
+    for (int x = tid + static_cast<int>(blockIdx.z) * kTileThreads; x < MN * 128; x += kTileThreads * p.splits) {
+      const int m = m0 + (x >> 7);
+      const long long n = static_cast<long long>(blockIdx.x) * 128 + (x & 127);
+      if (m >= p.m || n >= p.n) continue;
+      float v = 0.f;
+      for (int z = 0; z < p.splits; ++z) v += ld_cluster_f32(s_ring + static_cast<uint32_t>(x) * 4, static_cast<uint32_t>(z));
+      if (p.bias != nullptr) v += __ldg(p.bias + n);
+      uint8_t* y = p.y + (m * p.y_ld + n) * 2;
+      if (BF16) *reinterpret_cast<__nv_bfloat16*>(y) = __float2bfloat16_rn(v);
+      else *reinterpret_cast<__half*>(y) = __float2half_rn(v);
+    }
+    cluster_sync_all();                                             // the others have read this CTA's part
+  }
   if (tid == 0 && abort_word != 0 && p.status != nullptr) atomicCAS(p.status, 0, abort_word);
   if (warp == 1) tmem_dealloc(tmem, kTmemCols);
 }
@@ -648,9 +647,19 @@ struct Int4Op : Op {
     cudaGetDevice(&at);
     if (at != device) cudaSetDevice(device);
     if (x_pad != nullptr) int4_pad_rows<<<dim3((k8 + 255) / 256, p.m), 256, 0, s>>>(x_src, x_pad, x_src_ld, p.k, k8);
-    if (tile != nullptr) tile<<<grid, kTileThreads, smem, s>>>(tm_x, p);
-    else kernel<<<grid, kInt4Warps * 32, 0, s>>>(p);
-    const cudaError_t e = cudaGetLastError();
+    cudaError_t e = cudaSuccess;
+    if (tile != nullptr) {
+      cudaLaunchConfig_t cfg{};
+      cudaLaunchAttribute cluster{};
+      cfg.gridDim = grid; cfg.blockDim = dim3(kTileThreads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+      cluster.id = cudaLaunchAttributeClusterDimension;
+      cluster.val.clusterDim.x = 1; cluster.val.clusterDim.y = 1; cluster.val.clusterDim.z = p.splits;
+      cfg.attrs = &cluster; cfg.numAttrs = 1;
+      e = cudaLaunchKernelEx(&cfg, tile, tm_x, p);
+    } else {
+      kernel<<<grid, kInt4Warps * 32, smem, s>>>(p);
+    }
+    if (e == cudaSuccess) e = cudaGetLastError();
     if (at != device) cudaSetDevice(at);
     if (e != cudaSuccess) { set_error(std::string("int4 linear: ") + cudaGetErrorString(e)); return -1; }
     return 0;
@@ -663,31 +672,36 @@ bool group_ok(int g) { return g == 16 || g == 32 || g == 64 || g == 128 || g == 
 
 FDB_API int fdb_int4_desc_size() { return static_cast<int>(sizeof(Int4Desc)); }
 
+// Bytes of one packed block of 128 rows x 128 of K.
+static int int4_block_bytes(int scale_dtype, int group, bool zeros) {
+  const int per = 128 / std::min(group, 128);
+  return 8192 + 128 * per * (scale_dtype == kF32 ? 4 : 2) + (zeros ? 128 * std::max(1, per / 2) : 0);
+}
+
+FDB_API long long fdb_int4_packed_bytes(int scale_dtype, int has_zeros, int n, int k, int group) {
+  return static_cast<long long>((n + 127) / 128) * ((k + 127) / 128) * int4_block_bytes(scale_dtype, group, has_zeros != 0);
+}
+
 // Lays out a weight: q [n][groups][group / 2] bytes, scales [n][groups] (fp16, bf16 or fp32), zeros [n][(groups + 1) / 2]
-// bytes or null -> w [row tiles][k tiles][1024 bytes], out_scales and out_zeros as the product kernel reads them.
-FDB_API int fdb_int4_pack(const void* q, const void* scales, const void* zeros, void* w, void* out_scales, void* out_zeros,
-                          int scale_dtype, int n, int k, int group, void* stream) {
+// bytes or null -> blocks of 128 rows x 128 of K, fdb_int4_packed_bytes() in all.
+FDB_API int fdb_int4_pack(const void* q, const void* scales, const void* zeros, void* out, int scale_dtype, int n, int k,
+                          int group, void* stream) {
   if (!group_ok(group) || n < 1 || k < 1) { set_error("int4 pack: bad sizes"); return -1; }
-  if ((zeros == nullptr) != (out_zeros == nullptr)) { set_error("int4 pack: zeros and out_zeros come together"); return -1; }
+  if (scale_dtype != kF32 && scale_dtype != kF16 && scale_dtype != kBF16) { set_error("int4 pack: scales must be fp16, bf16 or fp32"); return -1; }
   const int k_tiles = (k + 127) / 128;
-  const long long tiles = static_cast<long long>((n + 15) / 16) * k_tiles;
+  const long long count = static_cast<long long>((n + 127) / 128) * k_tiles;
+  const long long bytes = int4_block_bytes(scale_dtype, group, zeros != nullptr);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const auto blocks = [](long long x) { return static_cast<int>(std::min<long long>((x + 255) / 256, 148 * 32)); };
-  int4_pack_weights<<<blocks(tiles * 256), 256, 0, s>>>(static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(zeros),
-                                                        static_cast<uint32_t*>(w), n, k, group, k_tiles, tiles * 256);
   const auto* z = static_cast<const uint8_t*>(zeros);
-  auto* oz = static_cast<uint8_t*>(out_zeros);
+  auto* o = static_cast<uint8_t*>(out);
+  int4_pack_weights<<<blocks(count * 2048), 256, 0, s>>>(static_cast<const uint8_t*>(q), z, o, n, k, group, k_tiles, bytes, count * 2048);
   if (scale_dtype == kF32)
-    int4_pack_scales<float><<<blocks(tiles * 16), 256, 0, s>>>(static_cast<const float*>(scales), z, static_cast<float*>(out_scales),
-                                                               oz, n, k, group, k_tiles, tiles * 16);
+    int4_pack_scales<float><<<blocks(count * 128), 256, 0, s>>>(static_cast<const float*>(scales), z, o, n, k, group, k_tiles, bytes, count * 128);
   else if (scale_dtype == kF16)
-    int4_pack_scales<__half><<<blocks(tiles * 16), 256, 0, s>>>(static_cast<const __half*>(scales), z, static_cast<__half*>(out_scales),
-                                                                oz, n, k, group, k_tiles, tiles * 16);
-  else if (scale_dtype == kBF16)
-    int4_pack_scales<__nv_bfloat16><<<blocks(tiles * 16), 256, 0, s>>>(static_cast<const __nv_bfloat16*>(scales), z,
-                                                                       static_cast<__nv_bfloat16*>(out_scales), oz, n, k, group,
-                                                                       k_tiles, tiles * 16);
-  else { set_error("int4 pack: scales must be fp16, bf16 or fp32"); return -1; }
+    int4_pack_scales<__half><<<blocks(count * 128), 256, 0, s>>>(static_cast<const __half*>(scales), z, o, n, k, group, k_tiles, bytes, count * 128);
+  else
+    int4_pack_scales<__nv_bfloat16><<<blocks(count * 128), 256, 0, s>>>(static_cast<const __nv_bfloat16*>(scales), z, o, n, k, group, k_tiles, bytes, count * 128);
   FDB_CUDA_OK(cudaGetLastError());
   return 0;
 }
@@ -712,30 +726,35 @@ FDB_API void* fdb_int4_linear_create(const Int4Desc* d) {
     p.x = static_cast<const uint8_t*>(d->x_pad); p.x_ld = op->k8;
   }
   p.y = static_cast<uint8_t*>(d->y); p.y_ld = d->y_ld; p.bias = d->bias;
-  p.w = static_cast<const uint4*>(d->w); p.scales = static_cast<const uint8_t*>(d->scales);
-  p.zeros = static_cast<const uint8_t*>(d->zeros);
+  p.w = static_cast<const uint8_t*>(d->w);
+  p.has_zeros = d->has_zeros;
+  p.block_bytes = static_cast<uint32_t>(int4_block_bytes(d->scale_dtype, d->group, d->has_zeros != 0));
   p.m = d->m; p.n = d->n; p.k_tiles = (d->k + 127) / 128;
   p.status = d->status;
   const int sg = 128 / std::min(d->group, 128);
-  const bool wide = d->scale_dtype == kF32, zero = d->zeros != nullptr;
+  const bool wide = d->scale_dtype == kF32, zero = d->has_zeros != 0;
   if (d->tile_rows == 0) {
     const int mt = d->m <= 8 ? 1 : 2;
     op->kernel = d->dtype == kBF16 ? pick<true>(wide, zero, sg, mt) : pick<false>(wide, zero, sg, mt);
     op->grid = dim3((d->n + 15) / 16, (d->m + 8 * mt - 1) / (8 * mt));
+    const int stage = 1024 + 16 * (sg * (wide ? 4 : 2) + (zero ? (sg >= 2 ? sg / 2 : 1) : 0));
+    op->smem = std::max(kInt4Warps * kVecStages * stage, kInt4Warps * 8 * mt * 16 * 4);
+    if (op->smem > 48 * 1024 &&
+        cudaFuncSetAttribute(reinterpret_cast<const void*>(op->kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, op->smem) != cudaSuccess) {
+      cudaGetLastError(); delete op; return fail("cannot raise the dynamic shared memory limit");
+    }
   } else {
     const int mn = d->tile_rows;
-    if ((mn != 16 && mn != 32 && mn != 64) || d->splits < 1 || d->splits > p.k_tiles ||
-        (d->splits > 1 && (d->partial == nullptr || d->counter == nullptr))) {
+    if ((mn != 16 && mn != 32 && mn != 64) || d->splits < 1 || d->splits > 8 || d->splits > p.k_tiles) {
       delete op; return fail("bad tile form");
     }
-    p.splits = d->splits; p.partial = d->partial; p.counter = d->counter;
+    p.splits = d->splits;
     op->tile = d->dtype == kBF16 ? pick_tile<true>(sg, mn) : pick_tile<false>(sg, mn);
     op->grid = dim3((d->n + 127) / 128, (d->m + mn - 1) / mn, d->splits);
-    const int scale_row = sg * (wide ? 4 : 2), zero_row = sg >= 2 ? sg / 2 : 1;
-    const int stage = (2 * mn * 128 + 8192 + 128 * (scale_row + zero_row) + 1023) / 1024 * 1024;
+    const int stage = (2 * mn * 128 + static_cast<int>(p.block_bytes) + 1023) / 1024 * 1024;
     p.wide = wide; p.stage_bytes = static_cast<uint32_t>(stage);
-    p.stages = std::min(kMaxInt4Stages, (227 * 1024 - 1024 - 1024 - 2 * 32768) / stage);
-    op->smem = 2 * 32768 + p.stages * stage + 1024;
+    p.stages = std::min(kMaxInt4Stages, (227 * 1024 - 1024 - 1024) / stage);
+    op->smem = p.stages * stage + 1024;
     EncodeTiledFn enc = get_encode_tiled();
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(d->k), static_cast<cuuint64_t>(d->m)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.x_ld) * 2};

@@ -393,6 +393,17 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The fp32 at this shared-memory address in CTA `rank` of the cluster.
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
+  float v;
+  asm volatile(
+      "{\n"
+      ".reg .b32 ra;\n"
+      "mapa.shared::cluster.u32 ra, %1, %2;\n"
+      "ld.shared::cluster.f32 %0, [ra];\n"
+      "}\n" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+  return v;
+}
 // Arrive on the mbarrier at the same shared-memory offset in CTA `rank` of the cluster. Relaxed: the
 // arrival hands back tensor memory whose reads this thread has already waited for (tcgen05.wait::ld); no
 // data written through the generic proxy travels with it, and a release here would first drain the

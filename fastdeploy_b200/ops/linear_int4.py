@@ -23,10 +23,9 @@ _SCALE_DTYPES = {torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.float32: 
 
 
 class _Int4Desc(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "y", "bias", "w", "scales", "zeros", "x_pad", "status", "partial",
-                                             "counter")] + \
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "y", "bias", "w", "x_pad", "status")] + \
                [("x_ld", ctypes.c_longlong), ("y_ld", ctypes.c_longlong)] + \
-               [(n, ctypes.c_int) for n in ("dtype", "scale_dtype", "m", "n", "k", "group", "tile_rows", "splits")]
+               [(n, ctypes.c_int) for n in ("dtype", "scale_dtype", "has_zeros", "m", "n", "k", "group", "tile_rows", "splits")]
 
 
 def _lib():
@@ -34,7 +33,9 @@ def _lib():
     if not getattr(lib, "_int4_ready", False):
         lib.fdb_int4_linear_create.restype = ctypes.c_void_p
         lib.fdb_int4_linear_create.argtypes = [ctypes.POINTER(_Int4Desc)]
-        lib.fdb_int4_pack.argtypes = [ctypes.c_void_p] * 6 + [ctypes.c_int] * 4 + [ctypes.c_void_p]
+        lib.fdb_int4_pack.argtypes = [ctypes.c_void_p] * 4 + [ctypes.c_int] * 4 + [ctypes.c_void_p]
+        lib.fdb_int4_packed_bytes.argtypes = [ctypes.c_int] * 5
+        lib.fdb_int4_packed_bytes.restype = ctypes.c_longlong
         if lib.fdb_int4_desc_size() != ctypes.sizeof(_Int4Desc):
             raise RuntimeError("libfdb200_kernels.so is out of date: Int4Desc layout differs; rebuild with "
                                "`python -m fastdeploy_b200._native.build`")
@@ -45,9 +46,9 @@ def _lib():
 @dataclass
 class Int4Weight:
     """A 4-bit weight ``[n, k]`` as the kernel reads it."""
-    data: torch.Tensor
-    scales: torch.Tensor
-    zeros: Optional[torch.Tensor]
+    data: torch.Tensor              # blocks of 128 rows x 128 columns: weights, scales, zero points
+    scale_dtype: torch.dtype
+    has_zeros: bool
     n: int
     k: int
     group: int
@@ -117,17 +118,14 @@ def pack_linear_weight_int4(qweight: torch.Tensor, scales: torch.Tensor, zero_po
     q, s = qweight.contiguous(), scales.contiguous()
     z = zero_points.contiguous() if zero_points is not None else None
     dev = q.device
-    tiles, per = -(-n // 16) * -(-k // 128), 128 // min(group, 128)
-    data = torch.empty(tiles * 1024, dtype=torch.uint8, device=dev)
-    out_s = torch.empty(tiles * 16 * per, dtype=s.dtype, device=dev)
-    out_z = torch.empty(tiles * 16 * max(1, per // 2), dtype=torch.uint8, device=dev) if z is not None else None
+    code = _SCALE_DTYPES[s.dtype]
+    data = torch.empty(_lib().fdb_int4_packed_bytes(code, int(z is not None), n, k, group), dtype=torch.uint8, device=dev)
     with torch.cuda.device(dev):
-        rc = _lib().fdb_int4_pack(q.data_ptr(), s.data_ptr(), z.data_ptr() if z is not None else None, data.data_ptr(),
-                                  out_s.data_ptr(), out_z.data_ptr() if out_z is not None else None,
-                                  _SCALE_DTYPES[s.dtype], n, k, group, ctypes.c_void_p(current_stream_ptr(dev)))
+        rc = _lib().fdb_int4_pack(q.data_ptr(), s.data_ptr(), z.data_ptr() if z is not None else None, data.data_ptr(), code,
+                                  n, k, group, current_stream_ptr(dev))
     if rc != 0:
         raise RuntimeError(f"int4 pack: {_native.last_error()}")
-    return Int4Weight(data, out_s, out_z, n, k, group)
+    return Int4Weight(data, s.dtype, z is not None, n, k, group)
 
 
 VECTOR_ROWS = 8
@@ -139,7 +137,7 @@ def _tile_form(m: int, weight: Int4Weight, sms: int) -> Tuple[int, int]:
         return 0, 1
     rows = 16 if m <= 16 else 32 if m <= 32 else 64
     ctas, k_tiles = -(-weight.n // 128) * -(-m // rows), -(-weight.k // 128)
-    return rows, max(1, min(sms // ctas, k_tiles // 4))
+    return rows, max(1, min(8, sms // ctas, k_tiles // 4))
 
 
 class Int4Linear(DeviceOp):
@@ -154,6 +152,8 @@ class Int4Linear(DeviceOp):
             raise ValueError(f"x has {x.shape[1]} columns and y {y.shape[1]}, the weight is {weight.n} x {weight.k}")
         if x.dtype not in _DTYPES or y.dtype != x.dtype:
             raise TypeError(f"x and y must both be fp16 or both bf16, got {x.dtype} and {y.dtype}")
+        if weight.scale_dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"the weight's scales are {weight.scale_dtype}: pack it with scales of {x.dtype} or fp32")
         m = x.shape[0]
         for what, t in (("x", x), ("y", y)):
             if t.stride(1) != 1 and t.shape[1] > 1:
@@ -170,22 +170,16 @@ class Int4Linear(DeviceOp):
         aligned = x.data_ptr() % 16 == 0 and d.x_ld % 8 == 0 and weight.k % 8 == 0
         # rows that 16-byte loads cannot take are copied to aligned ones first
         self.x_pad = None if aligned else torch.zeros(m, -(-weight.k // 8) * 8, dtype=x.dtype, device=x.device)
-        # the kernel reads scales of x's type or fp32; the other 16-bit type is widened, which changes no value
-        scales = weight.scales if weight.scales.dtype in (x.dtype, torch.float32) else weight.scales.float()
-        d.x, d.y, d.w, d.scales = x.data_ptr(), y.data_ptr(), weight.data.data_ptr(), scales.data_ptr()
+        d.x, d.y, d.w = x.data_ptr(), y.data_ptr(), weight.data.data_ptr()
         self.status = status or StatusWord(x.device)
         tile_rows, splits = _tile_form(m, weight, torch.cuda.get_device_properties(x.device).multi_processor_count)
-        columns = -(-weight.n // 128) * -(-m // max(1, tile_rows))
-        self.partial = torch.empty(splits, m, weight.n, dtype=torch.float32, device=x.device) if splits > 1 else None
-        self.counter = torch.zeros(columns, dtype=torch.int32, device=x.device) if splits > 1 else None
         d.tile_rows, d.splits, d.status = tile_rows, splits, self.status.ptr
-        for field, t in (("bias", bias), ("zeros", weight.zeros), ("x_pad", self.x_pad), ("partial", self.partial),
-                         ("counter", self.counter)):
+        for field, t in (("bias", bias), ("x_pad", self.x_pad)):
             setattr(d, field, t.data_ptr() if t is not None else None)
-        d.dtype, d.scale_dtype = _DTYPES[x.dtype], _SCALE_DTYPES[scales.dtype]
+        d.dtype, d.scale_dtype, d.has_zeros = _DTYPES[x.dtype], _SCALE_DTYPES[weight.scale_dtype], int(weight.has_zeros)
         d.m, d.n, d.k, d.group = m, weight.n, weight.k, weight.group
         super().__init__(lambda: _lib().fdb_int4_linear_create(ctypes.byref(d)),
-                         [x, y, bias, weight.data, scales, weight.zeros, self.x_pad, self.partial, self.counter, self.status], name, x.device)
+                         [x, y, bias, weight.data, self.x_pad, self.status], name, x.device)
         self.create = ("fdb_int4_linear_create", None, d)
 
 
