@@ -239,9 +239,10 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
           tma_load_4d(s_q + t * q_tile_bytes + c * chunk, &tm_q, bar_q, c * 64, 0, u.head, u.q_row + u.tok0 + t * p.tok);
     }
     bool ok = true;
-    for (int i = 0; ok && i < 2 * n_all; ++i) {
-      const int st = i % p.stages, round = i / p.stages;
-      if (round > 0) ok = mbar_wait_warp(bar(8 + st), (round - 1) & 1, abort_flag, kStatusTimeoutProducer);
+    RingAt at_ring{0, 0u};
+    for (int i = 0; ok && i < 2 * n_all; ++i, at_ring.step(1, p.stages)) {
+      const int st = at_ring.st;
+      if (i >= p.stages) ok = mbar_wait_warp(bar(8 + st), at_ring.parity ^ 1u, abort_flag, kStatusTimeoutProducer);
       if (!ok) break;
       const int j = i >> 1, row = u.k_row + (u.tile0 + j) * 128;
       const int keys = end_all - j * 128;
@@ -282,19 +283,19 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     if (lane == 0) {
       const uint32_t fmt = BF16 ? 1u : 0u;
       const uint32_t idesc_o = make_idesc(fmt, 128, static_cast<uint32_t>((p.D + 15) / 16 * 16)) | kIdescBMnMajor;
-      auto qk = [&](int t, int j) {
+      auto qk = [&](int t, int j, int st) {
         const int keys = min(128, key_end(t) - j * 128);
         const uint32_t idesc = make_idesc(fmt, 128, static_cast<uint32_t>((keys + 15) / 16 * 16));
-        const uint32_t sk = s_ring + static_cast<uint32_t>((2 * j) % p.stages) * stage_bytes;
+        const uint32_t sk = s_ring + static_cast<uint32_t>(st) * stage_bytes;
         for (int c = 0; c < p.d_chunks; ++c)
           umma_f16_ksteps(tmem + t * 128, make_kmajor_desc(s_q + t * q_tile_bytes + c * chunk, 128),
                           make_kmajor_desc(sk + c * chunk, 128), idesc, c != 0 ? 1u : 0u,
                           c + 1 == p.d_chunks ? static_cast<uint32_t>(p.d_steps_last) : 4u);
         umma_commit(bar_s(t));
       };
-      auto pv = [&](int t, int j) {
+      auto pv = [&](int t, int j, int st) {
         const int keys = min(128, key_end(t) - j * 128);
-        const uint64_t bd = make_mnmajor_desc(s_ring + static_cast<uint32_t>((2 * j + 1) % p.stages) * stage_bytes, chunk);
+        const uint64_t bd = make_mnmajor_desc(s_ring + static_cast<uint32_t>(st) * stage_bytes, chunk);
         for (int s = 0; s < (keys + 15) / 16; ++s)
           umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + s * 8, bd + static_cast<uint64_t>(s * 128), idesc_o,
                       (j | s) != 0 ? 1u : 0u);
@@ -303,25 +304,29 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       bool ok = mbar_wait(bar_q, 0, abort_flag, kStatusTimeoutMma) && mbar_wait(bar(0), 0, abort_flag, kStatusTimeoutMma);
       if (ok) {
         tc_fence_after();
-        for (int t = 0; t < 2; ++t) if (n_of(t) > 0) qk(t, 0);
+        for (int t = 0; t < 2; ++t) if (n_of(t) > 0) qk(t, 0, 0);
         umma_commit(bar(8));
       }
+      RingAt at_v{1, 0u};                                            // K_0 V_0 K_1 V_1 ... in the ring (three stages or more)
       for (int j = 0; ok && j < n_all; ++j) {
-        const int iv = 2 * j + 1, ik = 2 * j + 2;
-        ok = mbar_wait(bar(iv % p.stages), (iv / p.stages) & 1, abort_flag, kStatusTimeoutMma);
-        if (ok && j + 1 < n_all) ok = mbar_wait(bar(ik % p.stages), (ik / p.stages) & 1, abort_flag, kStatusTimeoutMma);
+        RingAt at_k = at_v;
+        at_k.step(1, p.stages);
+        ok = mbar_wait(bar(at_v.st), at_v.parity, abort_flag, kStatusTimeoutMma);
+        if (ok && j + 1 < n_all) ok = mbar_wait(bar(at_k.st), at_k.parity, abort_flag, kStatusTimeoutMma);
         for (int t = 0; ok && t < 2; ++t) {
           if (j >= n_of(t)) continue;
           ok = mbar_wait(bar_p(t), j & 1, abort_flag, kStatusTimeoutMma);
           if (!ok) break;
           tc_fence_after();
-          pv(t, j);
-          if (j + 1 < n_of(t)) qk(t, j + 1);
+          pv(t, j, at_v.st);
+          if (j + 1 < n_of(t)) qk(t, j + 1, at_k.st);
         }
         if (ok) {
-          umma_commit(bar(8 + iv % p.stages));
-          if (j + 1 < n_all) umma_commit(bar(8 + ik % p.stages));
+          umma_commit(bar(8 + at_v.st));
+          if (j + 1 < n_all) umma_commit(bar(8 + at_k.st));
         }
+        at_v = at_k;
+        at_v.step(1, p.stages);
       }
     }
     __syncwarp();

@@ -201,6 +201,7 @@ constexpr int kInt4Warps = 8;
 // Up to 8 MT rows of x; the CTA's eight warps share 16 weight rows, each warp a run of tiles along K, which it brings into
 // a ring of its own in shared memory by cp.async (no registers held, nothing to wait for but its own copies).
 constexpr int kVecStages = 4;
+template <bool V> struct WholeTile { static constexpr bool value = V; };
 
 template <bool BF16, bool WIDE, bool ZERO, int SG, int MT>
 __global__ void __launch_bounds__(kInt4Warps * 32)
@@ -215,56 +216,59 @@ int4_linear_kernel(const Int4Params p) {
   const int kt0 = p.k_tiles * warp / kInt4Warps, count = p.k_tiles * (warp + 1) / kInt4Warps - kt0;
   const int in_block = blockIdx.x & 7;                               // which 16 rows of a block
   const uint8_t* ring = ring_raw + warp * (kVecStages * kStage);
-  const uint32_t ring_at = smem_u32(ring);
-  const uint8_t* wp = p.w + (static_cast<long long>(blockIdx.x >> 3) * p.k_tiles + kt0) * p.block_bytes + lane * 16;
-  const uint32_t scales_at = 8192 + in_block * (16 * kScaleRow), zeros_at = 8192 + 128 * kScaleRow + in_block * (16 * kZeroRow);
-  auto fetch = [&](int i) {                                          // tile i of the warp; a group of copies either way
+  const uint32_t ring_at = smem_u32(ring) + lane * 16;
+  const uint8_t* wp = p.w + (static_cast<long long>(blockIdx.x >> 3) * p.k_tiles + kt0) * p.block_bytes + in_block * 1024 + lane * 16;
+  const uint32_t scales_at = 8192 + in_block * (16 * kScaleRow - 1024);        // from wp, like zeros_at
+  const uint32_t zeros_at = 8192 + 128 * kScaleRow + in_block * (16 * kZeroRow - 1024);
+  auto fetch = [&](int i, int stage) {                               // tile i of the warp; a group of copies either way
     if (i < count) {
-      const uint32_t at = ring_at + static_cast<uint32_t>(i % kVecStages) * kStage + lane * 16;
-      const uint8_t* block = wp + static_cast<long long>(i) * p.block_bytes;
-      cp_async_16(at, block + in_block * 1024, 16);
-      cp_async_16(at + 512, block + in_block * 1024 + 512, 16);
-      if (lane * 16 < 16 * kScaleRow) cp_async_16(at + 1024, block + scales_at, 16);
-      if (ZERO && lane * 16 < 16 * kZeroRow) cp_async_16(at + 1024 + 16 * kScaleRow, block + zeros_at, 16);
+      const uint32_t at = ring_at + static_cast<uint32_t>(stage) * kStage;
+      cp_async_16(at, wp, 16);
+      cp_async_16(at + 512, wp + 512, 16);
+      if (lane * 16 < 16 * kScaleRow) cp_async_16(at + 1024, wp + scales_at, 16);
+      if (ZERO && lane * 16 < 16 * kZeroRow) cp_async_16(at + 1024 + 16 * kScaleRow, wp + zeros_at, 16);
+      wp += p.block_bytes;
     }
     cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < kVecStages - 1; ++i) fetch(i);
+  for (int i = 0; i < kVecStages - 1; ++i) fetch(i, i);
 
   const uint8_t* xp[MT];
-  bool row_in[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    row_in[i] = m0 + i * 8 + g < p.m;
-    xp[i] = p.x + (row_in[i] ? (m0 + i * 8 + g) * p.x_ld * 2 : 0) + (kt0 * 128 + (SG == 8 ? 4 : 8) * t) * 2;
-  }
+  for (int i = 0; i < MT; ++i)
+    xp[i] = p.x + min(m0 + i * 8 + g, p.m - 1) * p.x_ld * 2 + (kt0 * 128 + (SG == 8 ? 4 : 8) * t) * 2;
   // Elements of x from this lane's first one to the end of the row: a load is made when it starts inside the row (K is a
   // multiple of 8 here, so it ends inside too).
   int left = p.k - kt0 * 128 - (SG == 8 ? 4 : 8) * t;
   const uint32_t piece_a = g * 64 + ((t + (g >> 1)) & 3) * 16;       // rows g and g + 8: the same place, 512 bytes apart
-  for (int i = 0; i < count; ++i, left -= 128) {
+  auto tile = [&](int i, auto whole_tag, int stage, int next_stage) {
+    constexpr bool whole = decltype(whole_tag)::value;
+    // Rows of x behind the last one repeat it: a column of the product that nobody stores. Only the row's last tile asks
+    // whether a load starts inside the row.
     uint4 xb[4][MT];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int r = 0; r < MT; ++r) {
-        xb[j][r] = make_uint4(0, 0, 0, 0);
         const uint8_t* a = xp[r] + j * 64;
         if (SG == 8) {
           // groups of 16: the lane's elements are 4 t .. of either group
-          if (row_in[r] && j * 32 < left) { const uint2 h = __ldg(reinterpret_cast<const uint2*>(a)); xb[j][r].x = h.x; xb[j][r].y = h.y; }
-          if (row_in[r] && j * 32 + 16 < left) { const uint2 h = __ldg(reinterpret_cast<const uint2*>(a + 32)); xb[j][r].z = h.x; xb[j][r].w = h.y; }
-        } else if (row_in[r] && j * 32 < left) {
-          xb[j][r] = __ldg(reinterpret_cast<const uint4*>(a));
+          uint2 h0 = make_uint2(0, 0), h1 = h0;
+          if (whole || j * 32 < left) h0 = __ldg(reinterpret_cast<const uint2*>(a));
+          if (whole || j * 32 + 16 < left) h1 = __ldg(reinterpret_cast<const uint2*>(a + 32));
+          xb[j][r] = make_uint4(h0.x, h0.y, h1.x, h1.y);
+        } else {
+          xb[j][r] = make_uint4(0, 0, 0, 0);
+          if (whole || j * 32 < left) xb[j][r] = __ldg(reinterpret_cast<const uint4*>(a));
         }
       }
 #pragma unroll
     for (int r = 0; r < MT; ++r) xp[r] += 256;
     cp_async_wait<kVecStages - 2>();
     __syncwarp();                                                    // every lane's copies of tile i have landed
-    fetch(i + kVecStages - 1);                                       // into the stage that tile i - 1 left
-    const uint8_t* at = ring + (i % kVecStages) * kStage;
+    fetch(i + kVecStages - 1, next_stage);                           // into the stage that tile i - 1 left
+    const uint8_t* at = ring + stage * kStage;
     const uint4 va = *reinterpret_cast<const uint4*>(at + piece_a), vb = *reinterpret_cast<const uint4*>(at + piece_a + 512);
     ScaleRow<BF16, WIDE, SG> s[2];
     s[0].load(at + 1024 + g * kScaleRow);
@@ -309,7 +313,15 @@ int4_linear_kernel(const Int4Params p) {
         }
       }
     }
+    left -= 128;
+  };
+  int i = 0;
+  const int whole = min(count, p.k / 128 - kt0);                     // tiles that end inside the row: the same for all lanes
+  for (; i + kVecStages <= whole; i += kVecStages) {
+#pragma unroll
+    for (int st = 0; st < kVecStages; ++st) tile(i + st, WholeTile<true>{}, st, (st + kVecStages - 1) % kVecStages);
   }
+  for (; i < count; ++i) tile(i, WholeTile<false>{}, i % kVecStages, (i + kVecStages - 1) % kVecStages);
   cp_async_wait<0>();
   __syncthreads();                                                   // the rings become the warps' sums
   constexpr int kCols = 8 * MT;
@@ -403,9 +415,10 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
     // ------------------------------------------------------------------------------------------------- producer
     bool ok = true;
     int issued = 0;
-    for (int it = 0; ok && it < n_it; ++it) {
-      const int st = it % p.stages, round = it / p.stages;
-      if (round > 0) ok = mbar_wait_warp(empty(st), (round - 1) & 1, abort_flag, kStatusTimeoutProducer);
+    RingAt at_ring{0, 0u};
+    for (int it = 0; ok && it < n_it; ++it, at_ring.step(1, p.stages)) {
+      const int st = at_ring.st;
+      if (it >= p.stages) ok = mbar_wait_warp(empty(st), at_ring.parity ^ 1u, abort_flag, kStatusTimeoutProducer);
       if (!ok) break;
       const uint32_t at = s_ring + static_cast<uint32_t>(st) * stage_bytes;
       if (lane == 0) {
@@ -427,9 +440,10 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
     if (lane == 0) {
       const uint32_t idesc = make_idesc(BF16 ? 1u : 0u, 128, MN);
       bool ok = true;
-      for (int it = 0; ok && it < n_it; ++it) {
-        const int st = it % p.stages, buf = it % kDequantGroups;
-        ok = mbar_wait(full(st), (it / p.stages) & 1, abort_flag, kStatusTimeoutMma) &&
+      RingAt at_ring{0, 0u};
+      for (int it = 0; ok && it < n_it; ++it, at_ring.step(1, p.stages)) {
+        const int st = at_ring.st, buf = it % kDequantGroups;
+        ok = mbar_wait(full(st), at_ring.parity, abort_flag, kStatusTimeoutMma) &&
              mbar_wait(a_full(buf), (it / kDequantGroups) & 1, abort_flag, kStatusTimeoutMma);
         const uint32_t ta = tmem + kA + buf * 64;
         const uint64_t bd = make_kmajor_desc(s_ring + static_cast<uint32_t>(st) * stage_bytes, 128);
@@ -457,9 +471,11 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
     // -------------------------------------------------------------------------------------------------- dequant
     const int group = (warp - 8) >> 2, r16 = row & 15;
     bool ok = true;
-    for (int it = group; ok && it < n_it; it += kDequantGroups) {
-      const int st = it % p.stages, round = it / kDequantGroups;
-      ok = mbar_wait_warp(full(st), (it / p.stages) & 1, abort_flag, kStatusTimeoutProducer);
+    RingAt at_ring{0, 0u};
+    at_ring.step(group, p.stages);
+    for (int it = group; ok && it < n_it; it += kDequantGroups, at_ring.step(kDequantGroups, p.stages)) {
+      const int st = at_ring.st, round = it / kDequantGroups;
+      ok = mbar_wait_warp(full(st), at_ring.parity, abort_flag, kStatusTimeoutProducer);
       if (!ok) break;
       const uint8_t* stage = ring + static_cast<uint32_t>(st) * stage_bytes;
       uint4 v[4];                                                   // v[t], word j: K elements j * 32 + 8 t ..
@@ -506,9 +522,10 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
   } else if (warp >= 4) {
     // ---------------------------------------------------------------------------------------------------- drain
     bool ok = true;
-    for (int it = 0; ok && it < n_it; ++it) {
-      const int st = it % p.stages;
-      ok = mbar_wait_warp(full(st), (it / p.stages) & 1, abort_flag, kStatusTimeoutProducer);
+    RingAt at_ring{0, 0u};
+    for (int it = 0; ok && it < n_it; ++it, at_ring.step(1, p.stages)) {
+      const int st = at_ring.st;
+      ok = mbar_wait_warp(full(st), at_ring.parity, abort_flag, kStatusTimeoutProducer);
       if (!ok) break;
       const uint8_t* sr = ring + static_cast<uint32_t>(st) * stage_bytes + kX + kW + row * scale_row;
       float s[SG];

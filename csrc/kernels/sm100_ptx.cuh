@@ -103,6 +103,15 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
   return __all_sync(0xffffffffu, ok) != 0;
 }
 
+// Position in a ring of stages and the parity of the round, advanced without a division.
+struct RingAt {
+  int st; uint32_t parity;
+  __device__ __forceinline__ void step(int by, int stages) {
+    st += by;
+    if (st >= stages) { st -= stages; parity ^= 1u; }
+  }
+};
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void prefetch_tensormap(const void* tmap) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tmap)) : "memory");
