@@ -280,7 +280,8 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     __syncwarp();
   } else if (warp == 8) {
     // ------------------------------------------------------------------------------------------------------------ MMA
-    if (lane == 0) {
+    // one elected thread: the compiler then keeps descriptors in uniform registers
+    if (elect_one()) {
       const uint32_t fmt = BF16 ? 1u : 0u;
       const uint32_t idesc_o = make_idesc(fmt, 128, static_cast<uint32_t>((p.D + 15) / 16 * 16)) | kIdescBMnMajor;
       auto qk = [&](int t, int j, int st) {

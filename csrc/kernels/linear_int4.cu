@@ -437,7 +437,9 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------------------------------------------------ MMA
-    if (lane == 0) {
+    // one elected thread: the compiler then keeps descriptors in uniform registers (with `lane == 0` it moved each operand
+    // of each MMA there on its own, 100 clocks an MMA)
+    if (elect_one()) {
       const uint32_t idesc = make_idesc(BF16 ? 1u : 0u, 128, MN);
       bool ok = true;
       RingAt at_ring{0, 0u};
