@@ -82,6 +82,29 @@ __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two fp32 at a time, in one 64-bit register pair.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void of_pair(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // What one CTA works on.
 struct Unit {
   int q_row;          // first row of the sequence in q / out (prefix form: 0)
@@ -103,7 +126,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const TileParams p) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 8];
+  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 10];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   __shared__ Unit unit;
@@ -183,12 +206,12 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   // 0..7 full, 8..15 empty, then:
   const uint32_t bar_q = bar(16), bar_tail = bar(17);
   auto bar_s = [&](int t) { return bar(18 + t); };
-  auto bar_p = [&](int t) { return bar(20 + t); };
-  auto bar_o = [&](int t) { return bar(22 + t); };
+  auto bar_o = [&](int t) { return bar(20 + t); };
+  auto bar_p = [&](int t, int half) { return bar(22 + 2 * t + half); };        // 64 keys each
   if (warp == 9 && lane == 0) {
     for (int i = 0; i < kMaxStages; ++i) { mbar_init(bar(i), 1); mbar_init(bar(8 + i), 1); }
     mbar_init(bar_q, 1); mbar_init(bar_tail, 1);
-    for (int t = 0; t < 2; ++t) { mbar_init(bar_s(t), 1); mbar_init(bar_p(t), 128); mbar_init(bar_o(t), 1); }
+    for (int t = 0; t < 2; ++t) { mbar_init(bar_s(t), 1); mbar_init(bar_o(t), 1); mbar_init(bar_p(t, 0), 4); mbar_init(bar_p(t, 1), 4); }
     fence_mbar_init();
     prefetch_tensormap(&tm_q); prefetch_tensormap(&tm_k); prefetch_tensormap(&tm_v);
   }
@@ -297,10 +320,21 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       auto pv = [&](int t, int j, int st) {
         const int keys = min(128, key_end(t) - j * 128);
         const uint64_t bd = make_mnmajor_desc(s_ring + static_cast<uint32_t>(st) * stage_bytes, chunk);
-        for (int s = 0; s < (keys + 15) / 16; ++s)
-          umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + s * 8, bd + static_cast<uint64_t>(s * 128), idesc_o,
-                      (j | s) != 0 ? 1u : 0u);
+        const int steps = (keys + 15) / 16;
+        // the second half of P is still being computed while the first one is multiplied
+        for (int half = 0; half < 2; ++half) {
+          if (!mbar_wait(bar_p(t, half), j & 1, abort_flag, kStatusTimeoutMma)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int s = half * 4 + x;
+            if (s < steps)
+              umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + s * 8, bd + static_cast<uint64_t>(s * 128), idesc_o,
+                          (j | s) != 0 ? 1u : 0u);
+          }
+        }
         umma_commit(bar_o(t));
+        return true;
       };
       bool ok = mbar_wait(bar_q, 0, abort_flag, kStatusTimeoutMma) && mbar_wait(bar(0), 0, abort_flag, kStatusTimeoutMma);
       if (ok) {
@@ -316,10 +350,8 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         if (ok && j + 1 < n_all) ok = mbar_wait(bar(at_k.st), at_k.parity, abort_flag, kStatusTimeoutMma);
         for (int t = 0; ok && t < 2; ++t) {
           if (j >= n_of(t)) continue;
-          ok = mbar_wait(bar_p(t), j & 1, abort_flag, kStatusTimeoutMma);
+          ok = pv(t, j, at_v.st);
           if (!ok) break;
-          tc_fence_after();
-          pv(t, j, at_v.st);
           if (j + 1 < n_of(t)) qk(t, j + 1, at_k.st);
         }
         if (ok) {
@@ -356,24 +388,24 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       const bool full = (j + 1) * 128 <= full_end;
       const int lim = row_end - j * 128;
       uint32_t v[4][32];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) if (b < blocks) tmem_ld_32x32(t_s + b * 32, v[b]);
-      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float m_new = m;
+      // the next 32 columns are on their way out of tensor memory while these are compared
+      tmem_ld_32x32(t_s, v[0]);
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         if (b >= blocks) continue;
-        if (b == 0) { tmem_ld_wait_dep(v[0]); }
-        if (b == 1) { tmem_ld_wait_dep(v[1]); }
-        if (b == 2) { tmem_ld_wait_dep(v[2]); }
-        if (b == 3) { tmem_ld_wait_dep(v[3]); }
+        tmem_ld_wait_dep(v[b]);
+        if (b < 3 && b + 1 < blocks) tmem_ld_32x32(t_s + (b + 1) * 32, v[(b + 1) & 3]);
         if (!full) {
 #pragma unroll
           for (int c = 0; c < 32; ++c) if (b * 32 + c >= lim) v[b][c] = 0xff800000u;      // minus infinity
         }
+        float m4[4] = {m_new, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 32; ++c) m4[c & 3] = fmaxf(m4[c & 3], __uint_as_float(v[b][c]));
+        for (int c = 0; c < 32; c += 2)
+          m4[(c >> 1) & 3] = max3(m4[(c >> 1) & 3], __uint_as_float(v[b][c]), __uint_as_float(v[b][c + 1]));
+        m_new = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
       }
-      const float m_new = fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
       const bool grow = m != -INFINITY && (m_new - m) * p.sl2 > kRescaleAbove;
       if (m == -INFINITY) m = m_new;
       if (__any_sync(0xffffffffu, grow)) {
@@ -394,32 +426,39 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         tmem_st_wait();
       }
       const float off = m == -INFINITY ? 0.f : -m * p.sl2;
-      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t scale2 = pair_of(p.sl2, p.sl2), off2 = pair_of(off, off);
+      uint64_t sum2[2] = {0, 0};                                     // zeros
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (2 * h >= blocks) continue;
-        uint32_t w[32];
+        if (2 * h < blocks) {
+          uint32_t w[32];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          if (2 * h + b < blocks) {
+          for (int b = 0; b < 2; ++b) {
+            if (2 * h + b < blocks) {
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const float e0 = exp2_ftz(fmaf(__uint_as_float(v[2 * h + b][2 * c]), p.sl2, off));
-              const float e1 = exp2_ftz(fmaf(__uint_as_float(v[2 * h + b][2 * c + 1]), p.sl2, off));
-              s4[c & 3] += e0 + e1;
-              w[b * 16 + c] = pack_pair<BF16>(e0, e1);
+              for (int c = 0; c < 16; ++c) {
+                float e0, e1;
+                of_pair(fma2(pair_of(__uint_as_float(v[2 * h + b][2 * c]), __uint_as_float(v[2 * h + b][2 * c + 1])), scale2, off2), e0, e1);
+                e0 = exp2_ftz(e0);
+                e1 = exp2_ftz(e1);
+                sum2[c & 1] = add2(sum2[c & 1], pair_of(e0, e1));
+                w[b * 16 + c] = pack_pair<BF16>(e0, e1);
+              }
+            } else {
+#pragma unroll
+              for (int c = 0; c < 16; ++c) w[b * 16 + c] = 0u;
             }
-          } else {
-#pragma unroll
-            for (int c = 0; c < 16; ++c) w[b * 16 + c] = 0u;
           }
+          tmem_st_32x32(t_s + h * 32, w);
+          tmem_st_wait();
         }
-        tmem_st_32x32(t_s + h * 32, w);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p(t, h));
       }
-      l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(bar_p(t));
+      float e0, e1;
+      of_pair(add2(sum2[0], sum2[1]), e0, e1);
+      l += e0 + e1;
     }
     if (ok && n > 0) {
       ok = mbar_wait(bar_o(t), (n - 1) & 1, abort_flag, kStatusTimeoutEpilogue);
