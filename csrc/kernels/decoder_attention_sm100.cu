@@ -540,16 +540,28 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
 }
 
 // One CTA: one item, one key head, up to 8 NT of its query heads, one split of the item's own keys. A warp takes 16 keys
-// at a time. Scores come transposed, S^T [16 keys x heads] = K Q^T, so that K rows are the A operand exactly as 16-byte
-// loads deliver them (the order of the head columns inside an MMA is free as long as Q follows it), and
-// O^T [head columns x heads] = V^T P takes V rows the same way after pairing two keys' halves with prmt: K and V never
-// pass through shared memory.
+// at a time, which it brings into a ring of its own in shared memory by cp.async, two tiles ahead (12 KB a warp in flight
+// for 128 columns; with the loads in registers and no tile ahead a 1024-key item ran at 3.3 TB/s). Scores come transposed,
+// S^T [16 keys x heads] = K Q^T, so that K rows are the A operand as 16-byte reads deliver them (the order of the head
+// columns inside an MMA is free as long as Q follows it), and O^T [head columns x heads] = V^T P takes V rows the same way
+// after pairing two keys' halves with prmt. Pieces of 16 bytes are permuted within a row by a function of the row, so that
+// both kinds of reads meet all banks.
+constexpr int kOwnStages = 3;
+
+__host__ __device__ constexpr int own_stage_bytes(int dp) { return 2 * 16 * dp * 2; }
+inline int own_smem_bytes(int dp, int nt, int parts) {
+  const int ring = kOwnWarps * kOwnStages * own_stage_bytes(dp);
+  const int join = (kOwnWarps * 8 * nt * dp + 8 * nt * (parts + kOwnWarps)) * 4;
+  return std::max(ring, join);
+}
+
 template <bool BF16, int DP, int NT>
 __global__ void __launch_bounds__(kOwnWarps * 32)
 own_keys_kernel(const OwnParams p) {
-  constexpr int KC = DP / 32, VC = DP / 64;
-  __shared__ float sm_o[kOwnWarps][8 * NT][DP];
+  constexpr int KC = DP / 32, VC = DP / 64, kRow = DP * 2, kUnits = DP / 8, kRowsAtOnce = 32 / kUnits;
+  extern __shared__ __align__(16) uint8_t own_smem[];
   __shared__ float2 sm_ml[kOwnWarps][8 * NT];
+  __shared__ float sm_inv[8 * NT];
   __shared__ unsigned ticket;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int column = blockIdx.x % p.columns, item = blockIdx.x / p.columns;
@@ -565,6 +577,32 @@ own_keys_kernel(const OwnParams p) {
   const int per = (((len + p.own_splits - 1) / p.own_splits) + 15) / 16 * 16;
   const int k0 = min(len, static_cast<int>(blockIdx.y) * per), k1 = min(len, k0 + per);
 
+  // ---- the warp's ring: tile i is keys k0 + (warp + kOwnWarps i) * 16 .. of K and of V
+  const uint8_t* ring = own_smem + warp * (kOwnStages * own_stage_bytes(DP));
+  const uint32_t ring_at = smem_u32(ring);
+  const uint8_t* kb = p.k + (item * p.k_item + static_cast<long long>(hk) * p.D) * 2;
+  const uint8_t* vb = p.v + (item * p.v_item + static_cast<long long>(hk) * p.D) * 2;
+  const int unit = lane % kUnits, row0 = lane / kUnits;
+  const bool unit_in = unit * 8 < p.D;
+  auto swizzle = [](int row) { return (((row >> 1) & 3) * 2) ^ ((row & 1) * 4); };
+  auto fetch = [&](int key, int stage) {
+    if (key < k1) {
+      const uint32_t at = ring_at + static_cast<uint32_t>(stage) * own_stage_bytes(DP);
+#pragma unroll
+      for (int i = 0; i < 16 / kRowsAtOnce; ++i) {
+        const int row = row0 + i * kRowsAtOnce;
+        const bool in = unit_in && key + row < k1;                  // what is not read is filled with zeros
+        const uint32_t to = at + row * kRow + (((unit & ~7) | ((unit & 7) ^ swizzle(row))) * 16);
+        cp_async_16(to, in ? kb + ((key + row) * p.k_ld + unit * 8) * 2 : kb, in ? 16 : 0);
+        cp_async_16(to + 16 * kRow, in ? vb + ((key + row) * p.v_ld + unit * 8) * 2 : vb, in ? 16 : 0);
+      }
+    }
+    cp_async_commit();
+  };
+  const int first = k0 + warp * 16;
+#pragma unroll
+  for (int i = 0; i < kOwnStages - 1; ++i) fetch(first + i * kOwnWarps * 16, i);
+
   uint4 q[NT][KC];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -579,71 +617,79 @@ own_keys_kernel(const OwnParams p) {
   float mx[NT][2], sum[NT][2];
 #pragma unroll
   for (int i = 0; i < NT; ++i) { mx[i][0] = mx[i][1] = -INFINITY; sum[i][0] = sum[i][1] = 0.f; }
-  const uint8_t* kb = p.k + (item * p.k_item + static_cast<long long>(hk) * p.D) * 2;
-  const uint8_t* vb = p.v + (item * p.v_item + static_cast<long long>(hk) * p.D) * 2;
 
-  for (int key = k0 + warp * 16; key < k1; key += kOwnWarps * 16) {
-    uint4 ka[KC], kc[KC], vv[4][VC];
-    const uint4 zero = make_uint4(0, 0, 0, 0);
+  int stage = 0;
+  for (int key = first; key < k1; key += kOwnWarps * 16) {
+    cp_async_wait<kOwnStages - 2>();
+    __syncwarp();                                                   // every lane's copies of this tile have landed
+    const int free_stage = stage == 0 ? kOwnStages - 1 : stage - 1; // the one that the previous tile left
+    fetch(key + (kOwnStages - 1) * kOwnWarps * 16, free_stage);
+    const uint8_t* at = ring + stage * own_stage_bytes(DP);
+    stage = stage + 1 == kOwnStages ? 0 : stage + 1;
+    float s[NT][4] = {};
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
-      const int d = c * 32 + t * 8;
-      ka[c] = kc[c] = zero;
-      if (d < p.D) {
-        if (key + g < k1) ka[c] = __ldg(reinterpret_cast<const uint4*>(kb + ((key + g) * p.k_ld + d) * 2));
-        if (key + g + 8 < k1) kc[c] = __ldg(reinterpret_cast<const uint4*>(kb + ((key + g + 8) * p.k_ld + d) * 2));
+      const int u = c * 4 + t, x = (u & ~7) | ((u & 7) ^ swizzle(g));
+      const uint4 ka = *reinterpret_cast<const uint4*>(at + g * kRow + x * 16);
+      const uint4 kc = *reinterpret_cast<const uint4*>(at + (g + 8) * kRow + x * 16);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        mma_16x8x16(s[i], ka.x, kc.x, ka.y, kc.y, q[i][c].x, q[i][c].y, BF16);
+        mma_16x8x16(s[i], ka.z, kc.z, ka.w, kc.w, q[i][c].z, q[i][c].w, BF16);
       }
     }
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int c = 0; c < VC; ++c) {
-        const int row = key + 2 * t + (x & 1) + (x >> 1) * 8, d = c * 64 + g * 8;
-        vv[x][c] = zero;
-        if (row < k1 && d < p.D) vv[x][c] = __ldg(reinterpret_cast<const uint4*>(vb + (row * p.v_ld + d) * 2));
-      }
+    // s[0], s[1]: key g, heads 2t and 2t + 1; s[2], s[3]: key g + 8
+    const bool in0 = key + g < k1, in1 = key + g + 8 < k1;
+    float a[NT][2];
+    uint32_t b0[NT], b1[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        mma_16x8x16(s, ka[c].x, kc[c].x, ka[c].y, kc[c].y, q[i][c].x, q[i][c].y, BF16);
-        mma_16x8x16(s, ka[c].z, kc[c].z, ka[c].w, kc[c].w, q[i][c].z, q[i][c].w, BF16);
-      }
-      // s[0], s[1]: key g, heads 2t and 2t + 1; s[2], s[3]: key g + 8
-      const bool in0 = key + g < k1, in1 = key + g + 8 < k1;
-      float e[4], a[2];
+      float e[4];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const float s0 = in0 ? s[x] * p.sl2 : -INFINITY, s1 = in1 ? s[2 + x] * p.sl2 : -INFINITY;
+        const float s0 = in0 ? s[i][x] * p.sl2 : -INFINITY, s1 = in1 ? s[i][2 + x] * p.sl2 : -INFINITY;
         float w = fmaxf(s0, s1);
         w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 4));
         w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 8));
         w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 16));
         w = fmaxf(w, mx[i][x]);
         const float base = w == -INFINITY ? 0.f : w;
-        a[x] = exp2_ftz(mx[i][x] - base);
+        a[i][x] = exp2_ftz(mx[i][x] - base);
         mx[i][x] = w;
         e[x] = exp2_ftz(s0 - base);
         e[2 + x] = exp2_ftz(s1 - base);
-        sum[i][x] = sum[i][x] * a[x] + e[x] + e[2 + x];
+        sum[i][x] = sum[i][x] * a[i][x] + e[x] + e[2 + x];
       }
-      const uint32_t b0 = transpose_8x8(pack_pair<BF16>(e[0], e[1])), b1 = transpose_8x8(pack_pair<BF16>(e[2], e[3]));
+      b0[i] = transpose_8x8(pack_pair<BF16>(e[0], e[1]));
+      b1[i] = transpose_8x8(pack_pair<BF16>(e[2], e[3]));
+    }
 #pragma unroll
-      for (int c = 0; c < VC; ++c) {
-        const uint32_t r0[4] = {vv[0][c].x, vv[0][c].y, vv[0][c].z, vv[0][c].w}, r1[4] = {vv[1][c].x, vv[1][c].y, vv[1][c].z, vv[1][c].w};
-        const uint32_t r2[4] = {vv[2][c].x, vv[2][c].y, vv[2][c].z, vv[2][c].w}, r3[4] = {vv[3][c].x, vv[3][c].y, vv[3][c].z, vv[3][c].w};
+    for (int c = 0; c < VC; ++c) {
+      uint4 vv[4];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+      for (int x = 0; x < 4; ++x) {
+        const int row = 2 * t + (x & 1) + (x >> 1) * 8;
+        vv[x] = *reinterpret_cast<const uint4*>(at + 16 * kRow + row * kRow + (c * 8 + (g ^ swizzle(row))) * 16);
+      }
+      const uint32_t r0[4] = {vv[0].x, vv[0].y, vv[0].z, vv[0].w}, r1[4] = {vv[1].x, vv[1].y, vv[1].z, vv[1].w};
+      const uint32_t r2[4] = {vv[2].x, vv[2].y, vv[2].z, vv[2].w}, r3[4] = {vv[3].x, vv[3].y, vv[3].z, vv[3].w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t a0 = __byte_perm(r0[w], r1[w], 0x5410), a1 = __byte_perm(r0[w], r1[w], 0x7632);
+        const uint32_t a2 = __byte_perm(r2[w], r3[w], 0x5410), a3 = __byte_perm(r2[w], r3[w], 0x7632);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
           float (&acc)[4] = o[i][2 * c + (w >> 1)][w & 1];
-          acc[0] *= a[0]; acc[1] *= a[1]; acc[2] *= a[0]; acc[3] *= a[1];
-          mma_16x8x16(acc, __byte_perm(r0[w], r1[w], 0x5410), __byte_perm(r0[w], r1[w], 0x7632),
-                      __byte_perm(r2[w], r3[w], 0x5410), __byte_perm(r2[w], r3[w], 0x7632), b0, b1, BF16);
+          acc[0] *= a[i][0]; acc[1] *= a[i][1]; acc[2] *= a[i][0]; acc[3] *= a[i][1];
+          mma_16x8x16(acc, a0, a1, a2, a3, b0[i], b1[i], BF16);
         }
       }
     }
   }
-  // ---- join the warps: sm_o[warp][head][column]
+  cp_async_wait<0>();
+  __syncthreads();                                                  // the rings become the warps' parts
+  float* sm_o = reinterpret_cast<float*>(own_smem);                 // [warp][head][column]
+  float* sm_w = sm_o + kOwnWarps * 8 * NT * DP;                     // [head][part]: weights of the parts that are joined
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
 #pragma unroll
@@ -660,32 +706,27 @@ own_keys_kernel(const OwnParams p) {
       for (int w = 0; w < 4; ++w)
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          sm_o[warp][i * 8 + 2 * t + (x & 1)][c * 64 + g * 8 + 2 * w + (x >> 1)] = o[i][2 * c + (w >> 1)][w & 1][x];
+          sm_o[(warp * 8 * NT + i * 8 + 2 * t + (x & 1)) * DP + c * 64 + g * 8 + 2 * w + (x >> 1)] = o[i][2 * c + (w >> 1)][w & 1][x];
   }
   __syncthreads();
   const int lanes_d = p.D / 4;                                      // a thread handles four columns of one head
   const bool single = p.own_splits == 1;
-  auto joined = [&](int h, int d, float& m, float& l) {
-    m = -INFINITY; l = 0.f;
-#pragma unroll
-    for (int w = 0; w < kOwnWarps; ++w) m = fmaxf(m, sm_ml[w][h].x);
-    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kOwnWarps; ++w) {
-      const float2 ml = sm_ml[w][h];
-      if (ml.y == 0.f) continue;                                    // no keys (a NaN sum goes on)
-      const float f = exp2_ftz(ml.x - m);
-      const float4 v = *reinterpret_cast<const float4*>(&sm_o[w][h][d]);
-      l += ml.y * f;
-      r.x += v.x * f; r.y += v.y * f; r.z += v.z * f; r.w += v.w * f;
-    }
-    return r;
-  };
   if (!single) {
     for (int x = threadIdx.x; x < heads * lanes_d; x += blockDim.x) {
       const int h = x / lanes_d, d = x % lanes_d * 4;
-      float m, l;
-      const float4 r = joined(h, d, m, l);
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kOwnWarps; ++w) m = fmaxf(m, sm_ml[w][h].x);
+      float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kOwnWarps; ++w) {
+        const float2 ml = sm_ml[w][h];
+        if (ml.y == 0.f) continue;                                  // no keys (a NaN sum goes on)
+        const float f = exp2_ftz(ml.x - m);
+        const float4 v = *reinterpret_cast<const float4*>(&sm_o[(w * 8 * NT + h) * DP + d]);
+        l += ml.y * f;
+        r.x += v.x * f; r.y += v.y * f; r.z += v.z * f; r.w += v.w * f;
+      }
       const long long row = (static_cast<long long>(blockIdx.y) * p.B + item) * p.H + head0 + h;
       *reinterpret_cast<float4*>(p.own_o + row * p.D + d) = r;
       if (d == 0) p.own_ml[row] = make_float2(m, l);
@@ -702,29 +743,54 @@ own_keys_kernel(const OwnParams p) {
   if (p.prefix_len != nullptr && prefix > 0) prefix = max(0, min(__ldg(p.prefix_len), prefix));
   const bool any_key = len > 0 || prefix > 0;
   wait_prerequisites();                                             // the prefix's parts
+  // ---- join: parts 0 .. own - 1 are this item's own (this CTA's warps, or the splits), the rest the prefix's. First a
+  // warp per head turns their maxima into weights, then each thread adds its columns of them, in order.
+  const int own = single ? kOwnWarps : p.own_splits, parts = own + p.splits;
+  auto part_row = [&](int s, int h) { return (static_cast<long long>(s) * p.B + item) * p.H + head0 + h; };
+  for (int h = warp; h < heads; h += kOwnWarps) {
+    auto stat = [&](int s) {
+      if (s >= own) return __ldcg(p.part_ml + part_row(s - own, h));
+      return single ? sm_ml[s][h] : __ldcg(p.own_ml + part_row(s, h));
+    };
+    float m = -INFINITY;
+    for (int s = lane; s < parts; s += 32) {
+      const float2 ml = stat(s);
+      if (ml.y != 0.f) m = fmaxf(m, ml.x);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    float l = 0.f;
+    for (int s = lane; s < parts; s += 32) {
+      const float2 ml = stat(s);
+      const float w = ml.y == 0.f ? 0.f : exp2_ftz(ml.x - m);
+      sm_w[h * parts + s] = w;
+      l += w == 0.f ? 0.f : w * ml.y;
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+    if (lane == 0) sm_inv[h] = any_key ? 1.f / l : 0.f;             // no key at all: zeros
+  }
+  __syncthreads();
   for (int x = threadIdx.x; x < heads * lanes_d; x += blockDim.x) {
     const int h = x / lanes_d, d = x % lanes_d * 4;
-    float m = -INFINITY, l = 0.f;
+    const float* weight = sm_w + h * parts;
     float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (single) r = joined(h, d, m, l);
-    auto add = [&](float2 ml, const float* src) {
-      if (ml.y == 0.f) return;
-      const float top = fmaxf(m, ml.x), fa = m == -INFINITY ? 0.f : exp2_ftz(m - top), fb = exp2_ftz(ml.x - top);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-      l = l * fa + ml.y * fb;
-      r.x = r.x * fa + v.x * fb; r.y = r.y * fa + v.y * fb; r.z = r.z * fa + v.z * fb; r.w = r.w * fa + v.w * fb;
-      m = top;
-    };
-    if (!single)
-      for (int s = 0; s < p.own_splits; ++s) {
-        const long long row = (static_cast<long long>(s) * p.B + item) * p.H + head0 + h;
-        add(__ldcg(p.own_ml + row), p.own_o + row * p.D + d);
+    if (single) {
+#pragma unroll
+      for (int w = 0; w < kOwnWarps; ++w) {
+        const float f = weight[w];
+        const float4 v = *reinterpret_cast<const float4*>(&sm_o[(w * 8 * NT + h) * DP + d]);
+        if (f != 0.f) { r.x += v.x * f; r.y += v.y * f; r.z += v.z * f; r.w += v.w * f; }
       }
-    for (int s = 0; s < p.splits; ++s) {
-      const long long row = (static_cast<long long>(s) * p.B + item) * p.H + head0 + h;
-      add(__ldcg(p.part_ml + row), p.part_o + row * p.D + d);
     }
-    const float inv = any_key ? 1.f / l : 0.f;                      // no key at all: zeros
+#pragma unroll 4
+    for (int s = single ? own : 0; s < parts; ++s) {
+      const float f = weight[s];
+      const float* src = s >= own ? p.part_o + part_row(s - own, h) * p.D + d : p.own_o + part_row(s, h) * p.D + d;
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+      if (f != 0.f) { r.x += v.x * f; r.y += v.y * f; r.z += v.z * f; r.w += v.w * f; }
+    }
+    const float inv = sm_inv[h];
     uint2 w;
     w.x = pack_pair<BF16>(r.x * inv, r.y * inv);
     w.y = pack_pair<BF16>(r.z * inv, r.w * inv);
@@ -771,7 +837,7 @@ struct DecoderAttnOp : Op {
   CUtensorMap tq, tk, tv;
   TileParams tile{};
   OwnParams own{};
-  int device = 0, tile_grid = 0, smem = 0, nt = 1;
+  int device = 0, tile_grid = 0, smem = 0, own_smem = 0, nt = 1;
   dim3 own_grid;
   bool bf16 = true, prefix = false, wide = false;
 
@@ -779,7 +845,7 @@ struct DecoderAttnOp : Op {
   cudaError_t dependent(K kernel, dim3 grid, int threads, cudaStream_t s, bool chained, const A&... args) {
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at{};
-    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.stream = s;
+    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = own_smem; cfg.stream = s;
     if (chained) {
       at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
       at.val.programmaticStreamSerializationAllowed = 1;
@@ -788,12 +854,12 @@ struct DecoderAttnOp : Op {
     return cudaLaunchKernelEx(&cfg, kernel, args...);
   }
   template <bool B>
+  void (*own_kernel())(const OwnParams) {
+    if (wide) return nt == 1 ? own_keys_kernel<B, 128, 1> : own_keys_kernel<B, 128, 2>;
+    return nt == 1 ? own_keys_kernel<B, 64, 1> : own_keys_kernel<B, 64, 2>;
+  }
   cudaError_t launch_own(cudaStream_t s) {
-    const bool chained = tile_grid > 0;
-    if (wide) return nt == 1 ? dependent(own_keys_kernel<B, 128, 1>, own_grid, kOwnWarps * 32, s, chained, own)
-                             : dependent(own_keys_kernel<B, 128, 2>, own_grid, kOwnWarps * 32, s, chained, own);
-    return nt == 1 ? dependent(own_keys_kernel<B, 64, 1>, own_grid, kOwnWarps * 32, s, chained, own)
-                   : dependent(own_keys_kernel<B, 64, 2>, own_grid, kOwnWarps * 32, s, chained, own);
+    return dependent(bf16 ? own_kernel<true>() : own_kernel<false>(), own_grid, kOwnWarps * 32, s, tile_grid > 0, own);
   }
   int launch(cudaStream_t s) override {
     int at = device;
@@ -809,7 +875,7 @@ struct DecoderAttnOp : Op {
       }
     }
     cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess && prefix) e = bf16 ? launch_own<true>(s) : launch_own<false>(s);
+    if (e == cudaSuccess && prefix) e = launch_own(s);
     if (at != device) cudaSetDevice(at);
     if (e != cudaSuccess) { set_error(std::string("decoder attention: ") + cudaGetErrorString(e)); return -1; }
     return 0;
@@ -911,6 +977,12 @@ FDB_API void* fdb_decoder_attention_create(const DecoderAttnDesc* d) {
       delete op; return fail("split own keys need their workspace");
     }
     op->own_grid = dim3(static_cast<unsigned>(o.columns) * d->rows, o.own_splits);
+    op->own_smem = own_smem_bytes(op->wide ? 128 : 64, op->nt, o.splits + o.own_splits);
+    if (op->own_smem > 227 * 1024 - 4096) { delete op; return fail("too many splits"); }
+    const void* fn = reinterpret_cast<const void*>(op->bf16 ? op->own_kernel<true>() : op->own_kernel<false>());
+    if (op->own_smem > 40 * 1024 && cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, op->own_smem) != cudaSuccess) {
+      cudaGetLastError(); delete op; return fail("cannot raise the dynamic shared memory limit");
+    }
   }
   return op;
 }
