@@ -55,7 +55,7 @@ struct TileParams {
   long long o_ld;
   int n_seq, rows, max_len;
   int H, Hk, G, D, tok;          // tok = 128 / G: tokens of one query tile
-  int causal, splits, tiles;     // prefix form: splits of the keys, pairs of query tiles
+  int causal, splits, tiles, wide_out;     // prefix form: splits of the keys, pairs of query tiles
   int d_chunks, d_steps_last, stages, units;
   uint32_t q_box_bytes;          // bytes of one Q chunk that TMA writes
   float sl2;                     // scale * log2 e
@@ -103,6 +103,13 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// 32 bytes, 32-byte aligned, in one store: a row's owner writes whole sectors.
+__device__ __forceinline__ void st_global_32(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f,
+                                             uint32_t g, uint32_t h) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e),
+               "r"(f), "r"(g), "r"(h) : "memory");
 }
 
 // What one CTA works on.
@@ -476,9 +483,9 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
           tmem_ld_wait_dep(o);
           if (real) {
 #pragma unroll
-            for (int c = 0; c < 32; c += 4)
+            for (int c = 0; c < 32; c += 8)
               if (c0 + c < p.D)
-                *reinterpret_cast<uint4*>(p.part_o + row * p.D + c0 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+                st_global_32(p.part_o + row * p.D + c0 + c, o[c], o[c + 1], o[c + 2], o[c + 3], o[c + 4], o[c + 5], o[c + 6], o[c + 7]);
           }
         }
       } else {
@@ -489,16 +496,21 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
           tmem_ld_32x32(t_o + c0, o);
           tmem_ld_wait_dep(o);
           if (real) {
+            uint32_t w[16];
 #pragma unroll
-            for (int c = 0; c < 32; c += 8)
-              if (c0 + c < p.D) {
-                uint4 w;
-                w.x = pack_pair<BF16>(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv);
-                w.y = pack_pair<BF16>(__uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv);
-                w.z = pack_pair<BF16>(__uint_as_float(o[c + 4]) * inv, __uint_as_float(o[c + 5]) * inv);
-                w.w = pack_pair<BF16>(__uint_as_float(o[c + 6]) * inv, __uint_as_float(o[c + 7]) * inv);
-                *reinterpret_cast<uint4*>(row + (c0 + c) * 2) = w;
+            for (int c = 0; c < 16; ++c)
+              w[c] = pack_pair<BF16>(__uint_as_float(o[2 * c]) * inv, __uint_as_float(o[2 * c + 1]) * inv);
+#pragma unroll
+            for (int c = 0; c < 32; c += 16) {
+              uint8_t* to = row + (c0 + c) * 2;
+              const uint32_t* x = w + c / 2;
+              if (p.wide_out) {                            // whole 32-byte sectors
+                if (c0 + c < p.D) st_global_32(to, x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+              } else {
+                if (c0 + c < p.D) *reinterpret_cast<uint4*>(to) = make_uint4(x[0], x[1], x[2], x[3]);
+                if (c0 + c + 8 < p.D) *reinterpret_cast<uint4*>(to + 16) = make_uint4(x[4], x[5], x[6], x[7]);
               }
+            }
           }
         }
       }
@@ -551,7 +563,7 @@ constexpr int kOwnStages = 3;
 __host__ __device__ constexpr int own_stage_bytes(int dp) { return 2 * 16 * dp * 2; }
 inline int own_smem_bytes(int dp, int nt, int parts) {
   const int ring = kOwnWarps * kOwnStages * own_stage_bytes(dp);
-  const int join = (kOwnWarps * 8 * nt * dp + 8 * nt * (parts + kOwnWarps)) * 4;
+  const int join = (kOwnWarps * 8 * nt * dp + 2 * 8 * nt * (parts + kOwnWarps)) * 4;
   return std::max(ring, join);
 }
 
@@ -568,6 +580,16 @@ own_keys_kernel(const OwnParams p) {
   const int chunks = p.columns / p.Hk, hk = column / chunks, h0 = column % chunks * (8 * NT);
   const int heads = min(8 * NT, p.G - h0);                          // query heads of this CTA
   const int head0 = hk * p.G + h0;
+  uint4 q[NT][KC];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const int h = i * 8 + g, d = c * 32 + t * 8;
+      q[i][c] = make_uint4(0, 0, 0, 0);
+      if (h < heads && d < p.D)
+        q[i][c] = __ldg(reinterpret_cast<const uint4*>(p.q + (item * p.q_ld + static_cast<long long>(head0 + h) * p.D + d) * 2));
+    }
   int len = p.own_rows;
   if (p.own_rows > 0) {
     const int n = __ldg(p.seq_len + item);
@@ -603,16 +625,6 @@ own_keys_kernel(const OwnParams p) {
 #pragma unroll
   for (int i = 0; i < kOwnStages - 1; ++i) fetch(first + i * kOwnWarps * 16, i);
 
-  uint4 q[NT][KC];
-#pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      const int h = i * 8 + g, d = c * 32 + t * 8;
-      q[i][c] = make_uint4(0, 0, 0, 0);
-      if (h < heads && d < p.D)
-        q[i][c] = __ldg(reinterpret_cast<const uint4*>(p.q + (item * p.q_ld + static_cast<long long>(head0 + h) * p.D + d) * 2));
-    }
   float o[NT][2 * VC][2][4] = {};       // [heads][64-column half: 4 m16 tiles as 2 x 2][..]: see the store below
   float mx[NT][2], sum[NT][2];
 #pragma unroll
@@ -690,6 +702,7 @@ own_keys_kernel(const OwnParams p) {
   __syncthreads();                                                  // the rings become the warps' parts
   float* sm_o = reinterpret_cast<float*>(own_smem);                 // [warp][head][column]
   float* sm_w = sm_o + kOwnWarps * 8 * NT * DP;                     // [head][part]: weights of the parts that are joined
+  float* sm_l = sm_w + 8 * NT * (p.splits + (p.own_splits == 1 ? kOwnWarps : p.own_splits));     // their sums
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
 #pragma unroll
@@ -755,16 +768,18 @@ own_keys_kernel(const OwnParams p) {
     float m = -INFINITY;
     for (int s = lane; s < parts; s += 32) {
       const float2 ml = stat(s);
+      sm_w[h * parts + s] = ml.x;
+      sm_l[h * parts + s] = ml.y;
       if (ml.y != 0.f) m = fmaxf(m, ml.x);
     }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
     float l = 0.f;
     for (int s = lane; s < parts; s += 32) {
-      const float2 ml = stat(s);
-      const float w = ml.y == 0.f ? 0.f : exp2_ftz(ml.x - m);
+      const float part_l = sm_l[h * parts + s];
+      const float w = part_l == 0.f ? 0.f : exp2_ftz(sm_w[h * parts + s] - m);
       sm_w[h * parts + s] = w;
-      l += w == 0.f ? 0.f : w * ml.y;
+      l += w == 0.f ? 0.f : w * part_l;
     }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
@@ -783,13 +798,23 @@ own_keys_kernel(const OwnParams p) {
         if (f != 0.f) { r.x += v.x * f; r.y += v.y * f; r.z += v.z * f; r.w += v.w * f; }
       }
     }
-#pragma unroll 4
-    for (int s = single ? own : 0; s < parts; ++s) {
-      const float f = weight[s];
-      const float* src = s >= own ? p.part_o + part_row(s - own, h) * p.D + d : p.own_o + part_row(s, h) * p.D + d;
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-      if (f != 0.f) { r.x += v.x * f; r.y += v.y * f; r.z += v.z * f; r.w += v.w * f; }
-    }
+    // eight parts' loads at a time are in flight
+    auto add = [&](const float* src, long long pitch, const float* w, int n) {
+      for (int s0 = 0; s0 < n; s0 += 8) {
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (s0 + k < n) v[k] = __ldcg(reinterpret_cast<const float4*>(src + (s0 + k) * pitch));
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float f = s0 + k < n ? w[s0 + k] : 0.f;
+          if (f != 0.f) { r.x += v[k].x * f; r.y += v[k].y * f; r.z += v[k].z * f; r.w += v[k].w * f; }
+        }
+      }
+    };
+    const long long pitch = static_cast<long long>(p.B) * p.H * p.D, at = part_row(0, h) * p.D + d;
+    if (!single) add(p.own_o + at, pitch, weight, own);
+    add(p.part_o + at, pitch, weight + own, p.splits);
     const float inv = sm_inv[h];
     uint2 w;
     w.x = pack_pair<BF16>(r.x * inv, r.y * inv);
@@ -925,6 +950,7 @@ FDB_API void* fdb_decoder_attention_create(const DecoderAttnDesc* d) {
   t.n_seq = d->n_seq; t.rows = d->rows; t.max_len = pf ? d->prefix_rows : std::min(d->max_len, d->rows);
   t.H = d->H; t.Hk = d->Hk; t.G = G; t.D = d->D; t.tok = 128 / G;
   t.causal = pf ? 0 : d->causal;
+  t.wide_out = reinterpret_cast<uintptr_t>(d->out) % 32 == 0 && d->o_ld % 16 == 0 && d->D % 16 == 0;
   t.splits = d->splits;
   t.d_chunks = (d->D + 63) / 64;
   t.d_steps_last = ((d->D - (t.d_chunks - 1) * 64) + 15) / 16;

@@ -199,11 +199,13 @@ class SharedPrefixAttention:
         self.status = status or StatusWord(dev)
         sms = torch.cuda.get_device_properties(dev).multi_processor_count
         group = heads // kv_heads
-        # The prefix is cut so that about every SM gets one piece of it, but no piece is shorter than a key tile.
+        # The prefix is cut until every SM has a piece of it, but no piece is shorter than four key tiles: each piece
+        # costs a launch of its own softmax and a part that the join reads (64 items, 4096 shared keys, 8 key heads of
+        # 128: 18 pieces 57 us, 8 pieces see the design notes).
         splits = 1
         if rows:
             pairs = -(-b // (2 * (128 // group)))
-            splits = max(1, min(-(-rows // KEY_TILE), sms // (pairs * kv_heads)))
+            splits = max(1, min(-(-rows // (4 * KEY_TILE)), sms // (pairs * kv_heads)))
         # Own keys: one CTA per item and key head reads up to 1024 keys; longer ones are cut while that adds CTAs to
         # idle SMs (four fit on one).
         per_head = 8 if group <= 8 else 16
