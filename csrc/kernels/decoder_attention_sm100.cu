@@ -55,7 +55,7 @@ struct TileParams {
   long long o_ld;
   int n_seq, rows, max_len;
   int H, Hk, G, D, tok;          // tok = 128 / G: tokens of one query tile
-  int causal, splits, tiles, wide_out;     // prefix form: splits of the keys, pairs of query tiles
+  int causal, splits, tiles;     // prefix form: splits of the keys, pairs of query tiles
   int d_chunks, d_steps_last, stages, units;
   uint32_t q_box_bytes;          // bytes of one Q chunk that TMA writes
   float sl2;                     // scale * log2 e
@@ -103,13 +103,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-
-// 32 bytes, 32-byte aligned, in one store: a row's owner writes whole sectors.
-__device__ __forceinline__ void st_global_32(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f,
-                                             uint32_t g, uint32_t h) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e),
-               "r"(f), "r"(g), "r"(h) : "memory");
 }
 
 // What one CTA works on.
@@ -473,45 +466,53 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     }
     if (ok && n > 0) {
       tc_fence_after();
+      // A thread owns a row, and rows are far apart in memory: stored from here, a warp's instruction would touch 32 lines
+      // (the fp32 parts of 256 rows of 128 took 9000 clocks). So a warp turns its 32 rows, 128 bytes of each at a time,
+      // around in the shared memory of this tile's queries, which the finished MMAs no longer read: eight threads then
+      // write a row's 128 bytes. Pieces of 16 bytes are permuted by the row, both ways without bank conflicts.
       const int head = u.head * p.G + r % p.G;
-      if (PREFIX) {
+      uint8_t* mine = nullptr;
+      if (real) {
         const long long row = (static_cast<long long>(u.split) * p.rows + token) * p.H + head;
-        if (real) p.part_ml[row] = make_float2(m == -INFINITY ? m : m * p.sl2, l);
-        for (int c0 = 0; c0 < p.D; c0 += 32) {
-          uint32_t o[32];
-          tmem_ld_32x32(t_o + c0, o);
-          tmem_ld_wait_dep(o);
-          if (real) {
+        if (PREFIX) p.part_ml[row] = make_float2(m == -INFINITY ? m : m * p.sl2, l);
+        mine = PREFIX ? reinterpret_cast<uint8_t*>(p.part_o + row * p.D)
+                      : p.out + ((static_cast<long long>(u.q_row) + token) * p.o_ld + static_cast<long long>(head) * p.D) * 2;
+      }
+      const float inv = PREFIX ? 1.f : 1.f / l;
+      const uint32_t turn = s_q + t * q_tile_bytes + static_cast<uint32_t>(warp & 3) * 4096u;
+      constexpr int kCols = PREFIX ? 32 : 64;                        // columns of O in 128 bytes
+      const int row_bytes = p.D * (PREFIX ? 4 : 2);
+      for (int c0 = 0; c0 < p.D; c0 += kCols) {
+        uint32_t w[32];
+        if (PREFIX) {
+          tmem_ld_32x32(t_o + c0, w);
+          tmem_ld_wait_dep(w);
+        } else {
 #pragma unroll
-            for (int c = 0; c < 32; c += 8)
-              if (c0 + c < p.D)
-                st_global_32(p.part_o + row * p.D + c0 + c, o[c], o[c + 1], o[c + 2], o[c + 3], o[c + 4], o[c + 5], o[c + 6], o[c + 7]);
-          }
-        }
-      } else {
-        const float inv = 1.f / l;
-        uint8_t* row = p.out + ((static_cast<long long>(u.q_row) + token) * p.o_ld + static_cast<long long>(head) * p.D) * 2;
-        for (int c0 = 0; c0 < p.D; c0 += 32) {
-          uint32_t o[32];
-          tmem_ld_32x32(t_o + c0, o);
-          tmem_ld_wait_dep(o);
-          if (real) {
-            uint32_t w[16];
+          for (int h = 0; h < 2; ++h) {
+            uint32_t o[32];
+            tmem_ld_32x32(t_o + c0 + h * 32, o);
+            tmem_ld_wait_dep(o);
 #pragma unroll
             for (int c = 0; c < 16; ++c)
-              w[c] = pack_pair<BF16>(__uint_as_float(o[2 * c]) * inv, __uint_as_float(o[2 * c + 1]) * inv);
-#pragma unroll
-            for (int c = 0; c < 32; c += 16) {
-              uint8_t* to = row + (c0 + c) * 2;
-              const uint32_t* x = w + c / 2;
-              if (p.wide_out) {                            // whole 32-byte sectors
-                if (c0 + c < p.D) st_global_32(to, x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
-              } else {
-                if (c0 + c < p.D) *reinterpret_cast<uint4*>(to) = make_uint4(x[0], x[1], x[2], x[3]);
-                if (c0 + c + 8 < p.D) *reinterpret_cast<uint4*>(to + 16) = make_uint4(x[4], x[5], x[6], x[7]);
-              }
-            }
+              w[h * 16 + c] = pack_pair<BF16>(__uint_as_float(o[2 * c]) * inv, __uint_as_float(o[2 * c + 1]) * inv);
           }
+        }
+        __syncwarp();                                                // the last 128 bytes have been read
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(turn + lane * 128 + ((c ^ (lane & 7)) << 4)),
+                       "r"(w[4 * c]), "r"(w[4 * c + 1]), "r"(w[4 * c + 2]), "r"(w[4 * c + 3]) : "memory");
+        __syncwarp();
+        const int at = c0 * (PREFIX ? 4 : 2) + (lane & 7) * 16;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int from = i * 4 + (lane >> 3);
+          uint8_t* to = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), from));
+          uint4 x;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                       : "r"(turn + from * 128 + (((lane & 7) ^ (from & 7)) << 4)) : "memory");
+          if (to != nullptr && at < row_bytes) *reinterpret_cast<uint4*>(to + at) = x;
         }
       }
     }
@@ -950,7 +951,6 @@ FDB_API void* fdb_decoder_attention_create(const DecoderAttnDesc* d) {
   t.n_seq = d->n_seq; t.rows = d->rows; t.max_len = pf ? d->prefix_rows : std::min(d->max_len, d->rows);
   t.H = d->H; t.Hk = d->Hk; t.G = G; t.D = d->D; t.tok = 128 / G;
   t.causal = pf ? 0 : d->causal;
-  t.wide_out = reinterpret_cast<uintptr_t>(d->out) % 32 == 0 && d->o_ld % 16 == 0 && d->D % 16 == 0;
   t.splits = d->splits;
   t.d_chunks = (d->D + 63) / 64;
   t.d_steps_last = ((d->D - (t.d_chunks - 1) * 64) + 15) / 16;
