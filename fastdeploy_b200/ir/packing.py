@@ -64,6 +64,8 @@ def pack_graph(graph: Graph, max_len: int) -> Graph:
     atts = [n for n in g.nodes if n.op == "Attention"]
     if not atts:
         raise PackingError("no fused Attention node: optimise the graph with static shapes first")
+    if any(n.attr("num_heads") is None for n in atts):
+        raise PackingError("a standard Attention node is not a fused encoder layer")
     masks = {n.inputs[3] if len(n.inputs) > 3 else "" for n in atts}
     if len(masks) > 1:
         raise PackingError("the attention layers do not share one mask")

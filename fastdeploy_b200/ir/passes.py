@@ -707,7 +707,7 @@ def fuse_qkv_gemms(graph: Graph) -> int:
     changed = 0
     cons = graph.consumers()
     prod = graph.producers()
-    for att in [n for n in graph.nodes if n.op in ("Attention", "PackedAttention")]:
+    for att in [n for n in graph.nodes if n.op in ("Attention", "PackedAttention") and n.attr("num_heads") is not None]:
         gemms = [prod.get(nm) for nm in att.inputs[:3]]
         if any(g is None or g.op != "FusedGemm" or len(g.inputs) != 3 for g in gemms) or len({id(g) for g in gemms}) != 3:
             continue

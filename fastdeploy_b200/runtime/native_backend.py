@@ -1220,8 +1220,84 @@ def _lower_EmbedLayerNorm(self: Lowering, node: Node):
     self.vals[node.outputs[0]] = Val(y.unflatten(0, out_shape[:-1]), False)
 
 
+def _lower_standard_attention(self: Lowering, node: Node):
+    """The standard ONNX operator over whole prompts, ``[B, S, heads * D]`` or ``[B, heads, S, D]``: every batch item is
+    a sequence of the packed kernel (ops/decoder.py). Masks, past keys, further outputs and a soft cap run elsewhere."""
+    from ..ops.decoder import CausalAttention
+    names = [nm for nm in node.inputs if nm]
+    shapes = [self.info.shapes[nm] for nm in node.inputs[:3]]
+    if len(names) != 3 or len([o for o in node.outputs if o]) != 1 or float(node.attr("softcap", 0.0)) > 0:
+        return False
+    flat = len(shapes[0]) == 3
+    if flat:
+        heads, kv_heads = int(node.attr("q_num_heads", 0)), int(node.attr("kv_num_heads", 0))
+        if heads < 1 or kv_heads < 1 or shapes[0][2] % heads:
+            return False
+        b, s, d = shapes[0][0], shapes[0][1], shapes[0][2] // heads
+        kv = [b, s, kv_heads * d]
+    else:
+        b, heads, s, d = shapes[0]
+        kv_heads = shapes[1][1]
+        kv = [b, kv_heads, s, d]
+    scale = float(node.attr("scale", 1.0 / math.sqrt(d)))
+    if shapes[1] != kv or shapes[2] != kv or d % 8 or d > 128 or heads % kv_heads or heads // kv_heads > 128 or scale <= 0:
+        return False
+
+    def rows(name, n):
+        if flat:
+            return self.rows_view(name, b * s, n * d)
+        buf = torch.zeros(b * s, n * d, dtype=self.dtype, device=self.device)
+        self.copy(self.as_torch(name), buf.view(b, s, n, d).permute(0, 2, 1, 3), f"rows({name})", node)
+        return buf
+    q, k, v = rows(node.inputs[0], heads), rows(node.inputs[1], kv_heads), rows(node.inputs[2], kv_heads)
+    out = torch.zeros(b * s, heads * d, dtype=self.dtype, device=self.device)
+    start = torch.arange(b, dtype=torch.int32, device=self.device) * s
+    att = CausalAttention(q, k, v, out, heads=heads, kv_heads=kv_heads, seq_start=start,
+                          seq_len=torch.full_like(start, s), max_len=s, scale=scale,
+                          causal=bool(node.attr("is_causal", 0)), status=self.plan.status)
+    for op in att.ops:
+        self.plan.add_native(op, node)
+        op.launch()
+    self.plan.extra.setdefault("attention", []).append(att)
+    y = out.view(b, s, heads * d) if flat else out.view(b, s, heads, d).permute(0, 2, 1, 3)
+    self.vals[node.outputs[0]] = Val(y, False)
+
+
+def _lower_MatMulNBits(self: Lowering, node: Node):
+    """A linear layer with 4-bit weights (ops/linear_int4.py); the weight is laid out once per plan builder."""
+    from ..ops.linear_int4 import GROUPS, Int4Linear, pack_linear_weight_int4
+    ins = list(node.inputs) + [""] * (6 - len(node.inputs))
+    n, k, group = int(node.attr("N", 0)), int(node.attr("K", 0)), int(node.attr("block_size", 0))
+    inits = self.g.initializers
+    if int(node.attr("bits", 4)) != 4 or group not in GROUPS or ins[4] or ins[1] not in inits or ins[2] not in inits:
+        return False
+    if ins[3] and (ins[3] not in inits or inits[ins[3]].dtype != np.uint8):
+        return False
+    shp = self.info.shapes[ins[0]]
+    if shp[-1] != k:
+        return False
+    rows, groups = _rows_of(shp), -(-k // group)
+    key = (ins[1], "int4")
+    if key not in self.packed:
+        scales = torch.from_numpy(np.ascontiguousarray(inits[ins[2]]))
+        scales = scales if scales.dtype == self.dtype else scales.float()      # fp16 scales of a bf16 plan: widened
+        zeros = torch.from_numpy(np.ascontiguousarray(inits[ins[3]])).to(self.device) if ins[3] else None
+        self.packed[key] = pack_linear_weight_int4(
+            torch.from_numpy(np.ascontiguousarray(inits[ins[1]])).view(n, groups, group // 2).to(self.device),
+            scales.to(self.device), zeros, k=k)
+    x2 = self.rows_view(ins[0], rows, k)
+    bias = self.const_f32(ins[5]).float().reshape(-1).contiguous() if ins[5] else None
+    y = torch.zeros(rows, _round8(n), dtype=self.dtype, device=self.device)
+    op = Int4Linear(x2, self.packed[key], y[:, :n], bias=bias, status=self.plan.status, name=f"int4:{node.name}")
+    self.plan.add_native(op, node)
+    op.launch()
+    self.vals[node.outputs[0]] = Val(y[:, :n].unflatten(0, shp[:-1]), False)
+
+
 def _lower_Attention(self: Lowering, node: Node):
     from ..ops.transformer import Attention
+    if node.attr("num_heads") is None:
+        return _lower_standard_attention(self, node)
     shp = self.info.shapes[node.inputs[0]]
     if len(shp) != 3:
         return False
@@ -1318,4 +1394,5 @@ Lowering.lower_LayerNormalization = _lower_LayerNormalization
 Lowering.lower_EmbedLayerNorm = _lower_EmbedLayerNorm
 Lowering.lower_Attention = _lower_Attention
 Lowering.lower_PackedAttention = _lower_PackedAttention
+Lowering.lower_MatMulNBits = _lower_MatMulNBits
 Lowering.lower_Gelu = _lower_Gelu

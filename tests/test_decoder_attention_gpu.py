@@ -175,3 +175,161 @@ def test_shared_prefix_attention(case, dtype):
         att.launch()
         att.status.check()
         check_prefix(q, pk, pv, k, v, lens, out, heads, kv_heads, d, 1 / math.sqrt(d))
+
+
+def test_lengths_are_read_at_launch_and_bad_ones_are_reported():
+    """One plan, several compositions, on a side stream and as a replayed graph; a sequence that does not fit its buffer is
+    left out and reported, the others are computed."""
+    from fastdeploy_b200.ops.decoder import CausalAttention
+    heads, kv_heads, d, rows = 4, 2, 64, 400
+    torch.manual_seed(3)
+    q, k, v = (torch.randn(rows, n * d, device="cuda").half() for n in (heads, kv_heads, kv_heads))
+    out = torch.empty(rows, heads * d, device="cuda", dtype=torch.float16)
+    start, lens = (torch.zeros(3, dtype=torch.int32, device="cuda") for _ in range(2))
+    att = CausalAttention(q, k, v, out, heads=heads, kv_heads=kv_heads, seq_start=start, seq_len=lens, max_len=300)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        att.launch()
+    for how, (st, ln) in enumerate([([0, 100, 399], [100, 299, 1]), ([5, 0, 0], [300, 0, 5]), ([10, 20, 300], [1, 200, 100])]):
+        start.copy_(torch.tensor(st)), lens.copy_(torch.tensor(ln)), out.fill_(7.0)
+        torch.cuda.synchronize()
+        if how == 0:
+            with torch.cuda.stream(side):
+                att.launch()
+        elif how == 1:
+            att.launch(side.cuda_stream)
+        else:
+            graph.replay()
+        torch.cuda.synchronize()
+        att.status.check()
+        check_packed(q, k, v, out, st, ln, heads, kv_heads, d, d ** -0.5, True, 7.0)
+    for st, ln, good in (([0, 390, 50], [20, 11, 10], [0, 2]), ([0, -1, 50], [20, 4, 10], [0, 2]), ([0, 60, 50], [20, -5, 10], [0, 2]),
+                         ([0, 60, 370], [20, 301, 30], [0, 2])):
+        start.copy_(torch.tensor(st)), lens.copy_(torch.tensor(ln)), out.fill_(7.0)
+        att.launch()
+        with pytest.raises(RuntimeError, match="bad shape"):
+            att.status.check()
+        check_packed(q, k, v, out, [st[i] for i in good], [ln[i] for i in good], heads, kv_heads, d, d ** -0.5, True, 7.0)
+
+
+def test_prefix_lengths_are_read_at_launch_and_cut_to_the_buffers():
+    from fastdeploy_b200.ops.decoder import SharedPrefixAttention
+    case = (4, 700, 50, [50, 0, 1, 20], 8, 2, 64)
+    q, pk, pv, k, v, length = make_prefix(case, torch.bfloat16, 4)
+    plen = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.empty(4, 512, device="cuda", dtype=torch.bfloat16)
+    att = SharedPrefixAttention(q, pk, pv, k, v, out, heads=8, kv_heads=2, seq_len=length, prefix_len=plen)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        att.launch()
+    for n in (700, 0, 1, 129, 512):
+        plen.fill_(n)
+        out.fill_(7.0)
+        graph.replay()
+        att.status.check()
+        check_prefix(q, pk[:n] if n else None, pv[:n], k, v, case[3], out, 8, 2, 64, 0.125)
+    plen.fill_(701)
+    att.launch()
+    with pytest.raises(RuntimeError, match="bad shape"):
+        att.status.check()
+    check_prefix(q, pk, pv, k, v, case[3], out, 8, 2, 64, 0.125)
+    plen.fill_(700)
+    k2, v2 = torch.nan_to_num(k), torch.nan_to_num(v)
+    k.copy_(k2), v.copy_(v2)
+    length.copy_(torch.tensor([51, -1, 1, 20]))
+    att.launch()
+    with pytest.raises(RuntimeError, match="bad shape"):
+        att.status.check()
+    check_prefix(q, pk, pv, k, v, [50, 0, 1, 20], out, 8, 2, 64, 0.125)
+
+
+def test_strided_caches_and_broadcast_items():
+    """Caches as [B, L] slices of a wider buffer, K and V interleaved, and one item's cache read by every item."""
+    from fastdeploy_b200.ops.decoder import SharedPrefixAttention
+    torch.manual_seed(5)
+    b, cap, hk, d, heads = 3, 37, 2, 96, 6
+    kv = torch.randn(b, 64, 2, hk * d, device="cuda").half()
+    k, v = kv[:, 10:10 + cap, 0], kv[:, 10:10 + cap, 1]
+    pkv = torch.randn(300, 2 * hk * d + 8, device="cuda").half()
+    pk, pv = pkv[:, :hk * d], pkv[:, hk * d:2 * hk * d]
+    qo = torch.randn(b, 2, heads * d, device="cuda").half()
+    lens = [37, 5, 16]
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    att = SharedPrefixAttention(qo[:, 0], pk, pv, k, v, qo[:, 1], heads=heads, kv_heads=hk, seq_len=length, scale=0.2)
+    att.launch()
+    att.status.check()
+    check_prefix(qo[:, 0], pk, pv, k, v, lens, qo[:, 1], heads, hk, d, 0.2)
+    one_k, one_v = k[:1].expand(b, -1, -1), v[:1].expand(b, -1, -1)
+    att = SharedPrefixAttention(qo[:, 0], pk, pv, one_k, one_v, qo[:, 1], heads=heads, kv_heads=hk, seq_len=length, scale=0.2)
+    att.launch()
+    check_prefix(qo[:, 0], pk, pv, one_k, one_v, lens, qo[:, 1], heads, hk, d, 0.2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_scores_rescale_and_equal_scores(dtype):
+    """Maxima that grow by far more than the rescaling threshold from tile to tile, and rows of equal scores."""
+    from fastdeploy_b200.ops.decoder import CausalAttention, SharedPrefixAttention
+    torch.manual_seed(6)
+    n, d = 700, 64
+    q = torch.randn(n, d, device="cuda").to(dtype)
+    ramp = torch.linspace(0, 4, n, device="cuda")[:, None]
+    k = (q.float().mean(0, keepdim=True) * 30 * ramp + torch.randn(n, d, device="cuda") * ramp).to(dtype)
+    v = torch.randn(n, d, device="cuda").to(dtype)
+    ints = [torch.tensor([x], dtype=torch.int32, device="cuda") for x in (0, n)]
+    for keys in (k, k.flip(0).contiguous(), torch.zeros_like(k)):
+        for causal in (True, False):
+            out = torch.empty_like(q)
+            CausalAttention(q, keys, v, out, heads=1, seq_start=ints[0], seq_len=ints[1], causal=causal).launch()
+            check_packed(q, keys, v, out, [0], [n], 1, 1, d, d ** -0.5, causal, 7.0)
+        out = torch.empty(1, d, dtype=dtype, device="cuda")
+        own = torch.tensor([n - 300], dtype=torch.int32, device="cuda")
+        SharedPrefixAttention(q[:1], keys[:300], v[:300], keys[None, 300:], v[None, 300:], out, heads=1, seq_len=own).launch()
+        check_prefix(q[:1], keys[:300], v[:300], keys[None, 300:], v[None, 300:], [n - 300], out, 1, 1, d, d ** -0.5)
+
+
+def test_prompt_then_decoding_steps_together():
+    """As a program uses them: a shared prompt goes through 4-bit projections and prompt attention, its keys become the
+    prefix; then three items decode five steps each, a captured step replayed, keys appended to their caches. Every
+    attention output is held against 64 bits over the very buffers it read."""
+    from fastdeploy_b200.ops.decoder import CausalAttention, SharedPrefixAttention
+    from fastdeploy_b200.ops.linear_int4 import Int4Linear, pack_linear_weight_int4, quantize_groups_int4
+    torch.manual_seed(7)
+    b, n, heads, hk, d, c, dt = 3, 150, 8, 2, 64, 512, torch.bfloat16
+    width = (heads + 2 * hk) * d
+    w = pack_linear_weight_int4(*quantize_groups_int4(torch.randn(width, c, device="cuda") * c ** -0.5, 32, symmetric=False))
+    x, qkv = torch.randn(n, c, device="cuda").to(dt), torch.empty(n, width, dtype=dt, device="cuda")
+    out = torch.empty(n, heads * d, dtype=dt, device="cuda")
+    q, pk, pv = qkv.split([heads * d, hk * d, hk * d], 1)
+    ints = [torch.tensor([z], dtype=torch.int32, device="cuda") for z in (0, n)]
+    proj = Int4Linear(x, w, qkv)
+    prompt = CausalAttention(q, pk, pv, out, heads=heads, kv_heads=hk, seq_start=ints[0], seq_len=ints[1])
+    proj.launch(), prompt.launch()
+    proj.status.check(), prompt.status.check()
+    check_packed(q, pk, pv, out, [0], [n], heads, hk, d, d ** -0.5, True, 7.0)
+
+    xs, step = torch.randn(b, c, device="cuda").to(dt), torch.empty(b, width, dtype=dt, device="cuda")
+    cache_k, cache_v = (torch.full((b, 6, hk * d), float("nan"), dtype=dt, device="cuda") for _ in range(2))
+    lens, o = torch.zeros(b, dtype=torch.int32, device="cuda"), torch.empty(b, heads * d, dtype=dt, device="cuda")
+    sq, sk, sv = step.split([heads * d, hk * d, hk * d], 1)
+    sproj = Int4Linear(xs, w, step)
+    att = SharedPrefixAttention(sq, pk, pv, cache_k, cache_v, o, heads=heads, kv_heads=hk, seq_len=lens)
+    at = torch.arange(b, device="cuda")
+
+    def one_step():
+        sproj.launch()
+        cache_k[at, lens.long()] = sk
+        cache_v[at, lens.long()] = sv
+        lens.add_(1)
+        att.launch()
+    one_step()
+    graph = torch.cuda.CUDAGraph()
+    check_prefix(sq, pk, pv, cache_k, cache_v, [1] * b, o, heads, hk, d, d ** -0.5)
+    with torch.cuda.graph(graph):
+        one_step()
+    for t in range(2, 6):
+        xs.copy_(torch.randn(b, c, device="cuda"))
+        graph.replay()
+        att.status.check(), sproj.status.check()
+        assert lens.tolist() == [t] * b
+        check_prefix(sq, pk, pv, cache_k, cache_v, [t] * b, o, heads, hk, d, d ** -0.5)
