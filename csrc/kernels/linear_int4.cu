@@ -348,10 +348,9 @@ int4_linear_kernel(const Int4Params p) {
 // From a few rows on, mma.sync (measured: 550 TFLOP/s) and the reads of x by every 16 weight rows cost more than the
 // weights' bytes. Here a CTA takes 128 weight rows as the M side of tcgen05.mma and MN rows of x as its N side:
 //   producer    one bulk copy of the packed block [128 x 128 of K] with its scales and zero points, TMA for x
-//   dequant     two groups of four warps take turns: q - z in 16 bits (exact), a weight row per thread, straight into
-//               tensor memory as the A operand (through shared memory it would be written and read back once per MMA:
-//               112 KB a tile in all, 900 clocks of the 128 bytes a clock; that form measured 80 us where this one's
-//               figure is in the table of the design notes' operator section)
+//   dequant     two groups of four warps take turns: q - z in 16 bits (exact), a weight row per thread,
+//               straight into tensor memory as the A operand (through shared memory it would be written and read back
+//               once per MMA: 112 KB a block in all, 900 clocks of the 128 bytes a clock)
 //   MMA         one product per scale group into one of four accumulators in tensor memory
 //   drain       four warps, a weight row per thread: sum += scale * accumulator, in fp32
 // so that the scales meet fp32 sums here too and the two kernels differ only in the order of their additions. Few weight
@@ -369,11 +368,14 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   constexpr uint32_t kX = 2 * MN * 128, kW = 8192;
+  // Blocks of a dequant turn: two halve the barrier round trips (16 rows, 14336 x 8192: 55 us with one, 37 with two); with
+  // 64 rows the drain's sums leave no registers for it (39 us with one, 41 with two).
+  constexpr int kTurn = MN == 64 ? 1 : 2;
   constexpr uint32_t kZeroRow = SG >= 2 ? SG / 2 : 1;
   const bool has_zeros = p.has_zeros != 0;
   const uint32_t scale_row = SG * (p.wide ? 4 : 2), stage_bytes = p.stage_bytes;
   constexpr uint32_t kA = 4 * MN;                                   // tensor memory: four accumulators, then A
-  constexpr uint32_t kTmemCols = kA + kDequantGroups * 64 <= 256 ? 256 : 512;
+  constexpr uint32_t kTmemCols = kA + kDequantGroups * kTurn * 64 <= 256 ? 256 : 512;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t s_ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint8_t* ring = smem_raw + (s_ring - smem_u32(smem_raw));
@@ -444,10 +446,10 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
       bool ok = true;
       RingAt at_ring{0, 0u};
       for (int it = 0; ok && it < n_it; ++it, at_ring.step(1, p.stages)) {
-        const int st = at_ring.st, buf = it % kDequantGroups;
+        const int st = at_ring.st, turn = it / kTurn, buf = turn % kDequantGroups, part = it % kTurn;
         ok = mbar_wait(full(st), at_ring.parity, abort_flag, kStatusTimeoutMma) &&
-             mbar_wait(a_full(buf), (it / kDequantGroups) & 1, abort_flag, kStatusTimeoutMma);
-        const uint32_t ta = tmem + kA + buf * 64;
+             (part != 0 || mbar_wait(a_full(buf), (turn / kDequantGroups) & 1, abort_flag, kStatusTimeoutMma));
+        const uint32_t ta = tmem + kA + (buf * kTurn + part) * 64;
         const uint64_t bd = make_kmajor_desc(s_ring + static_cast<uint32_t>(st) * stage_bytes, 128);
         for (int g = 0; ok && g < SG; ++g) {
           const int q = it * SG + g, d = q & 3;
@@ -463,7 +465,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
           umma_commit(d_full(d));
         }
         if (ok) {
-          umma_commit(a_empty(buf));
+          if (part == kTurn - 1 || it + 1 == n_it) umma_commit(a_empty(buf));
           umma_commit(empty(st));
         }
       }
@@ -474,9 +476,10 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
     const int group = (warp - 8) >> 2, r16 = row & 15;
     bool ok = true;
     RingAt at_ring{0, 0u};
-    at_ring.step(group, p.stages);
-    for (int it = group; ok && it < n_it; it += kDequantGroups, at_ring.step(kDequantGroups, p.stages)) {
-      const int st = at_ring.st, round = it / kDequantGroups;
+    at_ring.step(group * kTurn, p.stages);
+    for (int it0 = group * kTurn, round = 0; ok && it0 < n_it; it0 += kDequantGroups * kTurn, ++round) {
+     for (int it = it0; ok && it < min(it0 + kTurn, n_it); ++it) {
+      const int st = at_ring.st;
       ok = mbar_wait_warp(full(st), at_ring.parity, abort_flag, kStatusTimeoutProducer);
       if (!ok) break;
       const uint8_t* stage = ring + static_cast<uint32_t>(st) * stage_bytes;
@@ -488,7 +491,8 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
       if (has_zeros) z = load_zeros<SG>(stage + kX + kW + 128 * scale_row + row * kZeroRow);
       __syncwarp();
       if (lane == 0) mbar_arrive(empty(st));
-      if (round > 0) ok = mbar_wait_warp(a_empty(group), (round - 1) & 1, abort_flag, kStatusTimeoutMma);
+      at_ring.step(1, p.stages);
+      if (it == it0 && round > 0) ok = mbar_wait_warp(a_empty(group), (round - 1) & 1, abort_flag, kStatusTimeoutMma);
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
@@ -514,8 +518,11 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
             }
           }
         }
-        tmem_st_32x32(tmem + lanes + kA + group * 64 + half * 32, o);
+        tmem_st_32x32(tmem + lanes + kA + (group * kTurn + it - it0) * 64 + half * 32, o);
       }
+     }
+      if (!ok) break;
+      at_ring.step(kTurn, p.stages);                                // the other group's turn
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
