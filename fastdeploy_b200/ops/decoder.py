@@ -201,7 +201,7 @@ class SharedPrefixAttention:
         group = heads // kv_heads
         # The prefix is cut until every SM has a piece of it, but no piece is shorter than four key tiles: each piece
         # costs a launch of its own softmax and a part that the join reads (64 items, 4096 shared keys, 8 key heads of
-        # 128: 18 pieces 57 us, 8 pieces see the design notes).
+        # 128: 18 pieces 57 us, 8 pieces 42).
         splits = 1
         if rows:
             pairs = -(-b // (2 * (128 // group)))
