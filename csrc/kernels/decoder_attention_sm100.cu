@@ -990,7 +990,7 @@ FDB_API void* fdb_decoder_attention_create(const DecoderAttnDesc* d) {
                                     : reinterpret_cast<const void*>(&tile_attention_kernel<false, true>))
                         : (op->bf16 ? reinterpret_cast<const void*>(&tile_attention_kernel<true, false>)
                                     : reinterpret_cast<const void*>(&tile_attention_kernel<false, false>));
-    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, op->smem) != cudaSuccess) {
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynamicSmem) != cudaSuccess) {
       cudaGetLastError(); delete op; return fail("cannot raise the dynamic shared memory limit");
     }
   }
@@ -1011,9 +1011,9 @@ FDB_API void* fdb_decoder_attention_create(const DecoderAttnDesc* d) {
     }
     op->own_grid = dim3(static_cast<unsigned>(o.columns) * d->rows, o.own_splits);
     op->own_smem = own_smem_bytes(op->wide ? 128 : 64, op->nt, o.splits + o.own_splits);
-    if (op->own_smem > 227 * 1024 - 4096) { delete op; return fail("too many splits"); }
+    if (op->own_smem > kMaxDynamicSmem) { delete op; return fail("too many splits"); }
     const void* fn = reinterpret_cast<const void*>(op->bf16 ? op->own_kernel<true>() : op->own_kernel<false>());
-    if (op->own_smem > 40 * 1024 && cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, op->own_smem) != cudaSuccess) {
+    if (op->own_smem > 40 * 1024 && cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynamicSmem) != cudaSuccess) {
       cudaGetLastError(); delete op; return fail("cannot raise the dynamic shared memory limit");
     }
   }

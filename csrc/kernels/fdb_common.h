@@ -66,6 +66,10 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiledFn get_encode_tiled();
 
+// Dynamic shared memory that a kernel with up to 2 KB of static shared memory may be launched with. The limit belongs to the
+// function, not to a launch: plans of one kernel with different needs all set this one, so none lowers another's.
+constexpr int kMaxDynamicSmem = 227 * 1024 - 2048;
+
 // Number of SMs of the current device (cached per device).
 int sm_count();
 

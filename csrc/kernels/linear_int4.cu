@@ -769,7 +769,7 @@ FDB_API void* fdb_int4_linear_create(const Int4Desc* d) {
     const int stage = 1024 + 16 * (sg * (wide ? 4 : 2) + (zero ? (sg >= 2 ? sg / 2 : 1) : 0));
     op->smem = std::max(kInt4Warps * kVecStages * stage, kInt4Warps * 8 * mt * 16 * 4);
     if (op->smem > 48 * 1024 &&
-        cudaFuncSetAttribute(reinterpret_cast<const void*>(op->kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, op->smem) != cudaSuccess) {
+        cudaFuncSetAttribute(reinterpret_cast<const void*>(op->kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynamicSmem) != cudaSuccess) {
       cudaGetLastError(); delete op; return fail("cannot raise the dynamic shared memory limit");
     }
   } else {
@@ -794,7 +794,7 @@ FDB_API void* fdb_int4_linear_create(const Int4Desc* d) {
             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
       delete op; return fail("tensor map encoding failed");
     }
-    if (cudaFuncSetAttribute(reinterpret_cast<const void*>(op->tile), cudaFuncAttributeMaxDynamicSharedMemorySize, op->smem) != cudaSuccess) {
+    if (cudaFuncSetAttribute(reinterpret_cast<const void*>(op->tile), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynamicSmem) != cudaSuccess) {
       cudaGetLastError(); delete op; return fail("cannot raise the dynamic shared memory limit");
     }
   }

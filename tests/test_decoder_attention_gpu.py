@@ -333,3 +333,26 @@ def test_prompt_then_decoding_steps_together():
         att.status.check(), sproj.status.check()
         assert lens.tolist() == [t] * b
         check_prefix(sq, pk, pv, cache_k, cache_v, [t] * b, o, heads, hk, d, d ** -0.5)
+
+
+def test_plans_of_one_kernel_with_different_shared_memory():
+    """A later plan that needs less shared memory leaves an earlier one launchable."""
+    from fastdeploy_b200.ops.decoder import CausalAttention, SharedPrefixAttention
+    plans = []
+    for d in (128, 64):
+        q, k, v, start, length = make_packed([40], [0], 2, 2, d, torch.float16, 8)
+        out = torch.full((q.shape[0], 2 * d), 7.0, dtype=torch.float16, device="cuda")
+        plans.append((CausalAttention(q, k, v, out, heads=2, seq_start=start, seq_len=length), q, k, v, out, start, d))
+    for att, q, k, v, out, start, d in plans:
+        att.launch()
+        check_packed(q, k, v, out, start.tolist(), [40], 2, 2, d, d ** -0.5, True, 7.0)
+    plans = []
+    for cap in (120000, 300):                      # many splits of the own keys, then one
+        case = (1, 0, cap, [cap], 16, 1, 128)
+        q, pk, pv, k, v, length = make_prefix(case, torch.float16, 9)
+        out = torch.empty(1, 16 * 128, dtype=torch.float16, device="cuda")
+        plans.append((SharedPrefixAttention(q, pk, pv, k, v, out, heads=16, kv_heads=1, seq_len=length), q, k, v, cap, out))
+    for att, q, k, v, cap, out in plans:
+        att.launch()
+        att.status.check()
+        check_prefix(q, None, None, k, v, [cap], out, 16, 1, 128, 128 ** -0.5)

@@ -100,3 +100,17 @@ def test_quantised_weight_is_within_half_a_step():
         # half a step, and with zero points half a step more where rounding the zero point cuts the range's end
         assert ((back - w).abs() <= step * (0.5 if symmetric else 1.0) + 1e-6).all()
         check(linear_int4(x, pack_linear_weight_int4(q, s, z, k=300)), x, back, None)
+
+
+def test_plans_of_one_kernel_with_different_shared_memory():
+    """A later plan that needs less shared memory leaves an earlier one launchable."""
+    from fastdeploy_b200.ops.linear_int4 import Int4Linear, pack_linear_weight_int4
+    plans = []
+    for zero, scale_dtype in ((False, torch.bfloat16), (True, torch.float32), (False, torch.bfloat16)):
+        x, q, s, z = make(40, 130, 512, 16, zero, torch.bfloat16, scale_dtype)
+        y = torch.empty(40, 130, dtype=torch.bfloat16, device="cuda")
+        plans.append((Int4Linear(x, pack_linear_weight_int4(q, s, z), y), x, y, dense(q, s, z, 512)))
+    for op, x, y, w in plans:
+        op.launch()
+        op.status.check()
+        check(y, x, w, None)
