@@ -228,7 +228,7 @@ class Lowering(GenericLowering):
         self.plan = Plan(device)
         self.vals: Dict[str, Val] = {}
         self.consts: Dict[str, torch.Tensor] = {}
-        self.packed: Dict[Tuple[str, str], torch.Tensor] = {}
+        self.packed: Dict[Tuple, Any] = {}
         self.cons = graph.consumers()
         self.prod = graph.producers()
         self.preassigned: Dict[str, Val] = {}
@@ -1264,7 +1264,8 @@ def _lower_standard_attention(self: Lowering, node: Node):
 
 
 def _lower_MatMulNBits(self: Lowering, node: Node):
-    """A linear layer with 4-bit weights (ops/linear_int4.py); the weight is laid out once per plan builder."""
+    """A linear layer with 4-bit weights (ops/linear_int4.py); the weight is laid out once per plan builder and
+    set of scales and zero points."""
     from ..ops.linear_int4 import GROUPS, Int4Linear, pack_linear_weight_int4
     ins = list(node.inputs) + [""] * (6 - len(node.inputs))
     n, k, group = int(node.attr("N", 0)), int(node.attr("K", 0)), int(node.attr("block_size", 0))
@@ -1277,7 +1278,8 @@ def _lower_MatMulNBits(self: Lowering, node: Node):
     if shp[-1] != k:
         return False
     rows, groups = _rows_of(shp), -(-k // group)
-    key = (ins[1], "int4")
+    # nodes may share the weight and differ in all that is packed with it
+    key = (*ins[1:4], n, k, group, "int4")
     if key not in self.packed:
         scales = torch.from_numpy(np.ascontiguousarray(inits[ins[2]]))
         scales = scales if scales.dtype == self.dtype else scales.float()      # fp16 scales of a bf16 plan: widened
