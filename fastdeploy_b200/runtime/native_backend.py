@@ -1274,6 +1274,8 @@ def _lower_MatMulNBits(self: Lowering, node: Node):
         return False
     if ins[3] and (ins[3] not in inits or inits[ins[3]].dtype != np.uint8):
         return False
+    if ins[5] and ins[5] not in inits:
+        return False
     shp = self.info.shapes[ins[0]]
     if shp[-1] != k:
         return False

@@ -82,3 +82,15 @@ def test_a_weight_that_two_equal_nodes_share_is_laid_out_once(recorded):
     g.add_node("MatMulNBits", list(g.nodes[0].inputs), ["again"], domain="com.microsoft", N=N, K=K, bits=4, block_size=32)
     results, products, _ = recorded(g, {"x": [3, K]})
     assert results == [None, None] and products[0] is products[1]
+
+
+def test_a_computed_bias_is_left_to_the_interpreter(recorded):
+    g = shared_weight_graph((1.0, None, 32))
+    g.add_initializer("b0", np.ones(N, np.float32))
+    nodes = [["x", "w", "s0", "", "", b] for b in ("b0", "b")]
+    g.nodes.clear()
+    g.add_input("b", "float32", [N])
+    for i, ins in enumerate(nodes):
+        g.add_node("MatMulNBits", ins, [f"y{i}"], domain="com.microsoft", N=N, K=K, bits=4, block_size=32)
+    results, products, _ = recorded(g, {"x": [3, K]})
+    assert results == [None, False] and len(products) == 1
