@@ -86,12 +86,17 @@ def quantize_groups_int4(w: torch.Tensor, group: int = 128, symmetric: bool = Tr
     return packed.contiguous(), scale, (z[:, 0::2] | (z[:, 1::2] << 4)).contiguous()
 
 
+def _per_row(t: torch.Tensor, n: int, count: int) -> bool:
+    """Whether ``t`` holds ``count`` values for each of ``n`` rows: ``[n, count]`` (1s may follow) or flat."""
+    return t.numel() == n * count and (t.dim() == 1 or tuple(t.shape[:2]) == (n, count))
+
+
 def pack_linear_weight_int4(qweight: torch.Tensor, scales: torch.Tensor, zero_points: Optional[torch.Tensor] = None, *,
                             k: Optional[int] = None) -> Int4Weight:
     """Lays out ``qweight`` uint8 ``[n, groups, group // 2]`` (even element in the low half of a byte), ``scales``
     ``[n, groups]`` (fp16, bf16 or fp32, kept as they are) and ``zero_points`` uint8 ``[n, (groups + 1) // 2]`` (two to a
-    byte; ``None``: 8 everywhere) for the kernel. ``k`` is the weight's real column count when the last group is
-    partly padding."""
+    byte; ``None``: 8 everywhere) for the kernel; scales and zero points may also come flat. ``k`` is the weight's real
+    column count when the last group is partly padding."""
     if qweight.dim() != 3 or qweight.dtype != torch.uint8 or qweight.numel() == 0:
         raise ValueError(f"qweight: uint8 [n, groups, group // 2] is needed, got {qweight.dtype} {tuple(qweight.shape)}")
     n, groups, half = qweight.shape
@@ -103,12 +108,12 @@ def pack_linear_weight_int4(qweight: torch.Tensor, scales: torch.Tensor, zero_po
         raise ValueError(f"k = {k} does not fill {groups} groups of {group}")
     if scales.dtype not in _SCALE_DTYPES:
         raise TypeError(f"scales must be fp16, bf16 or fp32, got {scales.dtype}")
-    if scales.numel() != n * groups:
+    if not _per_row(scales, n, groups):
         raise ValueError(f"scales: {n} x {groups} values are needed, got {tuple(scales.shape)}")
     if zero_points is not None:
         if zero_points.dtype != torch.uint8:
             raise TypeError(f"zero points must be packed uint8, got {zero_points.dtype}")
-        if zero_points.numel() != n * ((groups + 1) // 2):
+        if not _per_row(zero_points, n, (groups + 1) // 2):
             raise ValueError(f"zero_points: {n} x {(groups + 1) // 2} bytes are needed, got {tuple(zero_points.shape)}")
     for name, t in (("scales", scales), ("zero_points", zero_points)):
         if t is not None and t.device != qweight.device:

@@ -1283,9 +1283,9 @@ def _lower_MatMulNBits(self: Lowering, node: Node):
     # nodes may share the weight and differ in all that is packed with it
     key = (*ins[1:4], n, k, group, "int4")
     if key not in self.packed:
-        scales = torch.from_numpy(np.ascontiguousarray(inits[ins[2]]))
+        scales = torch.from_numpy(np.ascontiguousarray(inits[ins[2]])).view(n, groups)
         scales = scales if scales.dtype == self.dtype else scales.float()      # fp16 scales of a bf16 plan: widened
-        zeros = torch.from_numpy(np.ascontiguousarray(inits[ins[3]])).to(self.device) if ins[3] else None
+        zeros = torch.from_numpy(np.ascontiguousarray(inits[ins[3]])).view(n, -1).to(self.device) if ins[3] else None
         self.packed[key] = pack_linear_weight_int4(
             torch.from_numpy(np.ascontiguousarray(inits[ins[1]])).view(n, groups, group // 2).to(self.device),
             scales.to(self.device), zeros, k=k)
