@@ -912,8 +912,9 @@ def fuse_embed_layernorm(graph: Graph) -> int:
 
 # --------------------------------------------------------------------------- pipelines
 def optimize(graph: Graph, input_shapes: Optional[Dict[str, Sequence[int]]] = None,
-             input_values: Optional[Dict[str, np.ndarray]] = None, level: int = 2) -> Graph:
-    """Runs the standard pipeline on a copy of ``graph``.
+             input_values: Optional[Dict[str, np.ndarray]] = None, level: int = 2, keep_qdq: bool = False) -> Graph:
+    """Runs the standard pipeline on a copy of ``graph``. ``keep_qdq`` leaves quantise / dequantise pairs where they are, for
+    an executor that computes in fp32 what they round and saturate.
 
     level 0: nothing; 1: constant folding and BN / bias folding (numerically safe rewrites);
     2: + operator fusion into FusedConv / FusedGemm / Attention / EmbedLayerNorm."""
@@ -934,7 +935,7 @@ def optimize(graph: Graph, input_shapes: Optional[Dict[str, Sequence[int]]] = No
         if not fold_constants(g, info):
             break
     hoist_dequantize_over_layout_ops(g)
-    if fold_qdq(g):
+    if not keep_qdq and fold_qdq(g):
         for _ in range(2):
             if not fold_constants(g, info):
                 break

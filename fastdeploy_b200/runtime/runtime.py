@@ -119,9 +119,10 @@ class Runtime:
             if self.option.cpu_thread_num > 0:
                 torch.set_num_threads(self.option.cpu_thread_num)
             # the CPU path runs the optimised graph (constant, batch-norm and bias folding, activations fused into
-            # their convolutions) with channel-innermost operands and weights packed once for the vendor primitive
+            # their convolutions) with channel-innermost operands and weights packed once for the vendor primitive;
+            # quantised exports keep their rounding and saturation
             from ..ir.passes import optimize
-            self._interp = Interpreter(optimize(self.graph, level=2), channels_last=True)
+            self._interp = Interpreter(optimize(self.graph, level=2, keep_qdq=True), channels_last=True)
 
     # ------------------------------------------------------------------ introspection
     def num_inputs(self) -> int:
