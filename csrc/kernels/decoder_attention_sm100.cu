@@ -172,7 +172,7 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         if (s < p.n_seq) {
           st = __ldg(p.seq_start + s);
           len = __ldg(p.seq_len + s);
-          if (len < 0 || len > p.max_len || st < 0 || st > p.rows - len) { bad = len != 0; len = 0; }
+          if (len < 0 || len > p.max_len || st < 0 || st > p.rows - len) { bad |= len != 0; len = 0; }
         }
         const int t = (len + 2 * p.tok - 1) / (2 * p.tok);
         int incl = t;
