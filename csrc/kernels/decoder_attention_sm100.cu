@@ -765,7 +765,9 @@ own_keys_kernel(const OwnParams p) {
   const bool any_key = len > 0 || prefix > 0;
   wait_prerequisites();                                             // the prefix's parts
   // ---- join: parts 0 .. own - 1 are this item's own (this CTA's warps, or the splits), the rest the prefix's. First a
-  // warp per head turns their maxima into weights, then each thread adds its columns of them, in order.
+  // warp per head turns their maxima into weights, then each thread adds its columns of them, in order. A part without a
+  // weight above zero (no keys, or none above minus infinity) gets the weight -1 and is left out: nobody may have written its
+  // columns. All others take part whatever their weight: a NaN reaches the result though its part's maximum is small.
   const int own = single ? kOwnWarps : p.own_splits, parts = own + p.splits;
   auto part_row = [&](int s, int h) { return (static_cast<long long>(s) * p.B + item) * p.H + head0 + h; };
   for (int h = warp; h < heads; h += kOwnWarps) {
@@ -785,9 +787,9 @@ own_keys_kernel(const OwnParams p) {
     float l = 0.f;
     for (int s = lane; s < parts; s += 32) {
       const float part_l = sm_l[h * parts + s];
-      const float w = part_l == 0.f ? 0.f : exp2_ftz(sm_w[h * parts + s] - m);
+      const float w = part_l == 0.f ? -1.f : exp2_ftz(sm_w[h * parts + s] - m);
       sm_w[h * parts + s] = w;
-      l += w == 0.f ? 0.f : w * part_l;
+      if (part_l != 0.f) l += w * part_l;
     }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
@@ -803,7 +805,7 @@ own_keys_kernel(const OwnParams p) {
       for (int w = 0; w < kOwnWarps; ++w) {
         const float f = weight[w];
         const float4 v = *reinterpret_cast<const float4*>(&sm_o[(w * 8 * NT + h) * DP + d]);
-        if (f != 0.f) { r.x += v.x * f; r.y += v.y * f; r.z += v.z * f; r.w += v.w * f; }
+        if (!(f < 0.f)) { r.x += v.x * f; r.y += v.y * f; r.z += v.z * f; r.w += v.w * f; }
       }
     }
     // eight parts' loads at a time are in flight
@@ -815,8 +817,8 @@ own_keys_kernel(const OwnParams p) {
           if (s0 + k < n) v[k] = __ldcg(reinterpret_cast<const float4*>(src + (s0 + k) * pitch));
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float f = s0 + k < n ? w[s0 + k] : 0.f;
-          if (f != 0.f) { r.x += v[k].x * f; r.y += v[k].y * f; r.z += v[k].z * f; r.w += v[k].w * f; }
+          const float f = s0 + k < n ? w[s0 + k] : -1.f;
+          if (!(f < 0.f)) { r.x += v[k].x * f; r.y += v[k].y * f; r.z += v[k].z * f; r.w += v[k].w * f; }
         }
       }
     };
