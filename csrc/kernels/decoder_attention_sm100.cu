@@ -11,12 +11,16 @@
 //
 //   S = Q K^T   (operands in shared memory, fp32 accumulator in tensor memory)
 //   P = 2^(...) rounded to the inputs' 16-bit type and written over S in tensor memory (the A operand of the next MMA;
-//               the row sum l is taken from the unrounded fp32 values, so P's rounding, half a step of the 16-bit type
-//               each, is the only one between the inputs and the output's own)
+//               the row sum l is taken from the unrounded fp32 values, so P's rounding is the only one between the inputs
+//               and the output's own: half a step of the 16-bit type each, 2^-8 (bf16) or 2^-11 of the weight, because the
+//               tensor cores multiply 16-bit operands; P in two 16-bit parts would double the second product)
 //   O += P V    (V as it lies in memory, keys by head columns: an MN-major operand, no transpose)
 //
 // The maximum a row is scaled by only moves when it grew by more than 8 in log2 units: until then p <= 2^8, which the
-// 16-bit types and the fp32 sums hold without loss, and O needs no rescaling.
+// 16-bit types and the fp32 sums hold without loss, and O needs no rescaling. fp16 has fixed steps of 2^-24 below 2^-14,
+// which would take small weights away that together count (32768 weights of 2^-25 were lost to the last one), so fp16 weights
+// are held 2^7 times as large (at most 2^15): below 2^-21 a weight is off by at most 2^-32, all of up to 2^20 keys together by
+// 2^-12 of the largest. l and O carry the same factor, which the quotient does not see.
 //
 // One 16384-token causal sequence, 16 query heads over 4 of 128 columns, bf16: 1054 us, 1.04 PFLOP/s (1.4 is what a long
 // cuBLAS product sustains). A pair of tiles takes 3500 clocks a key tile where the products need 2048 and the exponential
@@ -75,6 +79,10 @@ constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 constexpr int kMaxStages = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleAbove = 8.f;   // log2 units
+// log2 of the factor that 16-bit weights are held with (bf16 has fp32's range and needs none): for p <= 2^8, and for the own
+// keys, whose maximum never lags, for p <= 1.
+template <bool BF16> constexpr float kTileUp = BF16 ? 0.f : 7.f;
+template <bool BF16> constexpr float kOwnUp = BF16 ? 0.f : 15.f;
 
 __device__ __forceinline__ float exp2_ftz(float x) {
   float y;
@@ -432,7 +440,7 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         }
         tmem_st_wait();
       }
-      const float off = m == -INFINITY ? 0.f : -m * p.sl2;
+      const float off = m == -INFINITY ? 0.f : kTileUp<BF16> - m * p.sl2;
       const uint64_t scale2 = pair_of(p.sl2, p.sl2), off2 = pair_of(off, off);
       uint64_t sum2[2] = {0, 0};                                     // zeros
 #pragma unroll
@@ -481,7 +489,7 @@ tile_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       uint8_t* mine = nullptr;
       if (real) {
         const long long row = (static_cast<long long>(u.split) * p.rows + token) * p.H + head;
-        if (PREFIX) p.part_ml[row] = make_float2(m == -INFINITY ? m : m * p.sl2, l);
+        if (PREFIX) p.part_ml[row] = make_float2(m == -INFINITY ? m : m * p.sl2 - kTileUp<BF16>, l);
         mine = PREFIX ? reinterpret_cast<uint8_t*>(p.part_o + row * p.D)
                       : p.out + ((static_cast<long long>(u.q_row) + token) * p.o_ld + static_cast<long long>(head) * p.D) * 2;
       }
@@ -673,8 +681,8 @@ own_keys_kernel(const OwnParams p) {
         w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 8));
         w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 16));
         w = fmaxf(w, mx[i][x]);
-        const float base = w == -INFINITY ? 0.f : w;
-        a[i][x] = exp2_ftz(mx[i][x] - base);
+        const float top = w == -INFINITY ? 0.f : w, base = top - kOwnUp<BF16>;
+        a[i][x] = exp2_ftz(mx[i][x] - top);
         mx[i][x] = w;
         e[x] = exp2_ftz(s0 - base);
         e[2 + x] = exp2_ftz(s1 - base);
@@ -719,7 +727,7 @@ own_keys_kernel(const OwnParams p) {
       w += __shfl_xor_sync(0xffffffffu, w, 4);
       w += __shfl_xor_sync(0xffffffffu, w, 8);
       w += __shfl_xor_sync(0xffffffffu, w, 16);
-      if (g == 0) sm_ml[warp][i * 8 + 2 * t + x] = make_float2(mx[i][x], w);
+      if (g == 0) sm_ml[warp][i * 8 + 2 * t + x] = make_float2(mx[i][x] - kOwnUp<BF16>, w);
     }
 #pragma unroll
     for (int c = 0; c < VC; ++c)
