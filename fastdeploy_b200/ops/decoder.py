@@ -95,6 +95,20 @@ def _pitch(t: torch.Tensor, dim: int, least: int) -> int:
     return t.stride(dim) if t.shape[dim] > 1 else (least + 7) // 8 * 8
 
 
+def _own_splits(own: int, ctas: int, d: int, sms: int) -> int:
+    """Pieces that an item's own keys are cut into, from the rows of its cache (the lengths are only known on the device).
+
+    Uncut, a CTA reads all own keys of an item and key head (of up to 16 query heads). Where such CTAs leave SMs without
+    work, caches of 512 rows or more are cut, into pieces of at least 256 rows, until every SM has one CTA, or two of heads
+    of up to 64 columns, whose rings hold half the bytes. That is half of what fits on an SM (98 and 49 KB of shared memory
+    a CTA): the ring of one CTA keeps enough bytes on their way, and each further piece is a part that goes through memory
+    and is joined. 128 columns, one CTA an SM against four: 1 item, 8 key heads, 32768 keys 48 and 54 us; 1 item, 1 key
+    head of 16 query heads, 120000 keys 81 and 200 us; 4 items, 8 key heads, 16384 keys 72 and 77 us. 64 columns, two
+    against four: 1 item, 12 key heads, 32768 keys 41 and 44 us (one: 43)."""
+    per_sm = 1 if d > 64 else 2
+    return max(1, min(own // 256, per_sm * sms // ctas))
+
+
 def _make(desc: _DecoderAttnDesc, keep, name: str, device: torch.device) -> DeviceOp:
     op = DeviceOp(lambda: _lib().fdb_decoder_attention_create(ctypes.byref(desc)), keep, name, device)
     op.create = ("fdb_decoder_attention_create", None, desc)
@@ -206,11 +220,9 @@ class SharedPrefixAttention:
         if rows:
             pairs = -(-b // (2 * (128 // group)))
             splits = max(1, min(-(-rows // (4 * KEY_TILE)), sms // (pairs * kv_heads)))
-        # Own keys: one CTA per item and key head reads up to 1024 keys; longer ones are cut while that adds CTAs to
-        # idle SMs (four fit on one).
         per_head = 8 if group <= 8 else 16
         columns = kv_heads * -(-group // per_head)
-        own_splits = max(1, min(own // 256, (4 * sms) // (b * columns))) if own else 1
+        own_splits = _own_splits(own, b * columns, d, sms)
 
         def space(*shape, dtype=torch.float32):
             return torch.zeros(*shape, dtype=dtype, device=dev)
