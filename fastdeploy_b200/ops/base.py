@@ -68,6 +68,14 @@ class NativeOp:
             pass
 
 
+def settle(device: torch.device) -> None:
+    """Waits for the fills of a new plan's workspace, which the allocation queued on ``device``'s current stream: the plan may
+    be launched on another one next. During a capture they become part of the graph, which such a plan belongs to."""
+    with torch.cuda.device(device):
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(device).synchronize()
+
+
 class DeviceOp(NativeOp):
     """A native op that runs on the device of its tensors, whichever device is current: ``create`` is called with that
     device current, and a launch without a stream goes to that device's current stream."""

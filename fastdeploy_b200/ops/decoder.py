@@ -6,8 +6,8 @@
 
 Both are planned over fixed buffers like the operators of :mod:`.transformer`; the lengths are device tensors that every
 launch reads, so that one plan (and one CUDA graph) serves every batch composition that fits the buffers. A plan owns its
-workspace: launches of one plan have to be ordered (one stream, or streams that wait for one another); two plans are
-independent.
+workspace, which is ready on every stream when the constructor returns (one made during a graph capture is that graph's):
+launches of one plan have to be ordered (one stream, or streams that wait for one another); two plans are independent.
 """
 from __future__ import annotations
 
@@ -18,7 +18,7 @@ from typing import Optional
 import torch
 
 from .. import _native
-from .base import DT_BF16, DT_F16, DeviceOp, StatusWord
+from .base import DT_BF16, DT_F16, DeviceOp, StatusWord, settle
 
 KEY_TILE = 128          # keys per tile of the tensor-core kernel
 
@@ -112,6 +112,7 @@ def _own_splits(own: int, ctas: int, d: int, sms: int) -> int:
 def _make(desc: _DecoderAttnDesc, keep, name: str, device: torch.device) -> DeviceOp:
     op = DeviceOp(lambda: _lib().fdb_decoder_attention_create(ctypes.byref(desc)), keep, name, device)
     op.create = ("fdb_decoder_attention_create", None, desc)
+    settle(device)
     return op
 
 

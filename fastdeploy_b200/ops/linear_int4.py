@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native
-from .base import DT_BF16, DT_F16, DT_F32, DeviceOp, StatusWord, current_stream_ptr
+from .base import DT_BF16, DT_F16, DT_F32, DeviceOp, StatusWord, current_stream_ptr, settle
 
 GROUPS = (16, 32, 64, 128, 256)
 _DTYPES = {torch.float16: DT_F16, torch.bfloat16: DT_BF16}
@@ -150,6 +150,7 @@ def _tile_form(m: int, weight: Int4Weight, sms: int) -> Tuple[int, int]:
 class Int4Linear(DeviceOp):
     """Planned ``y[M, n] = x[M, k] @ W^T + bias`` over fixed buffers: ``x`` and ``y`` fp16 or bf16 with any row pitch,
     ``bias`` fp32 ``[n]``."""
+    _any_stream = True
 
     def __init__(self, x: torch.Tensor, weight: Int4Weight, y: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
                  status: Optional[StatusWord] = None, name: str = "int4_linear"):
@@ -175,8 +176,8 @@ class Int4Linear(DeviceOp):
         d = _Int4Desc()
         d.x_ld, d.y_ld = (x.stride(0), y.stride(0)) if m > 1 else (-(-weight.k // 8) * 8, weight.n)
         aligned = x.data_ptr() % 16 == 0 and d.x_ld % 8 == 0 and weight.k % 8 == 0
-        # rows that 16-byte loads cannot take are copied to aligned ones first
-        self.x_pad = None if aligned else torch.zeros(m, -(-weight.k // 8) * 8, dtype=x.dtype, device=x.device)
+        # rows that 16-byte loads cannot take are copied to aligned ones first (every launch writes all of them)
+        self.x_pad = None if aligned else torch.empty(m, -(-weight.k // 8) * 8, dtype=x.dtype, device=x.device)
         d.x, d.y, d.w = x.data_ptr(), y.data_ptr(), weight.data.data_ptr()
         self.status = status or StatusWord(x.device)
         tile_rows, splits = _tile_form(m, weight, torch.cuda.get_device_properties(x.device).multi_processor_count)
@@ -188,10 +189,17 @@ class Int4Linear(DeviceOp):
         super().__init__(lambda: _lib().fdb_int4_linear_create(ctypes.byref(d)),
                          [x, y, bias, weight.data, self.x_pad, self.status], name, x.device)
         self.create = ("fdb_int4_linear_create", None, d)
+        if self._any_stream:
+            settle(x.device)
+
+
+class _SameStream(Int4Linear):
+    """A product that is launched on the stream it was made on, which orders its workspace: nothing to wait for."""
+    _any_stream = False
 
 
 def linear_int4(x: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Eager ``x @ W^T + bias`` for ``x`` ``[M, k]``."""
     y = torch.empty(x.shape[0], weight.n, dtype=x.dtype, device=x.device)
-    Int4Linear(x, weight, y, bias=bias.float().contiguous() if bias is not None else None).launch()
+    _SameStream(x, weight, y, bias=bias.float().contiguous() if bias is not None else None).launch()
     return y
