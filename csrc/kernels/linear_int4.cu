@@ -110,11 +110,13 @@ __global__ void int4_pack_scales(const S* __restrict__ s, const uint8_t* __restr
   }
 }
 
-// x with rows that 16-byte loads cannot take -> rows of k rounded up to 8, zeros behind k.
+// x with rows that 16-byte loads cannot take -> rows of k rounded up to 8, zeros behind k. Rows are the grid's x, which may
+// have 2^31 - 1 of them (y ends at 65535).
+constexpr int kPadThreads = 256;
 __global__ void int4_pad_rows(const uint16_t* __restrict__ x, uint16_t* __restrict__ out, long long x_ld, int k, int k8) {
-  const uint16_t* row = x + blockIdx.y * x_ld;
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c < k8) out[static_cast<long long>(blockIdx.y) * k8 + c] = c < k ? row[c] : uint16_t(0);
+  const uint16_t* row = x + blockIdx.x * x_ld;
+  uint16_t* to = out + static_cast<long long>(blockIdx.x) * k8;
+  for (int c = blockIdx.y * kPadThreads + threadIdx.x; c < k8; c += gridDim.y * kPadThreads) to[c] = c < k ? row[c] : uint16_t(0);
 }
 
 // ---------------------------------------------------------------------------------------------------------- product
@@ -675,9 +677,14 @@ struct Int4Op : Op {
     int at = device;
     cudaGetDevice(&at);
     if (at != device) cudaSetDevice(device);
-    if (x_pad != nullptr) int4_pad_rows<<<dim3((k8 + 255) / 256, p.m), 256, 0, s>>>(x_src, x_pad, x_src_ld, p.k, k8);
     cudaError_t e = cudaSuccess;
-    if (tile != nullptr) {
+    if (x_pad != nullptr) {
+      int4_pad_rows<<<dim3(p.m, std::min((k8 + kPadThreads - 1) / kPadThreads, 1024)), kPadThreads, 0, s>>>(x_src, x_pad, x_src_ld, p.k, k8);
+      e = cudaGetLastError();
+    }
+    if (e != cudaSuccess) {
+      // without its rows the product has nothing to read
+    } else if (tile != nullptr) {
       cudaLaunchConfig_t cfg{};
       cudaLaunchAttribute cluster{};
       cfg.gridDim = grid; cfg.blockDim = dim3(kTileThreads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
