@@ -373,14 +373,11 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   constexpr uint32_t kX = 2 * MN * 128, kW = 8192;
-  // Blocks of a dequant turn: two halve the barrier round trips (16 rows, 14336 x 8192: 55 us with one, 37 with two); with
-  // 64 rows the drain's sums leave no registers for it (39 us with one, 41 with two).
-  constexpr int kTurn = MN == 64 ? 1 : 2;
   constexpr uint32_t kZeroRow = SG >= 2 ? SG / 2 : 1;
   const bool has_zeros = p.has_zeros != 0;
   const uint32_t scale_row = SG * (p.wide ? 4 : 2), stage_bytes = p.stage_bytes;
   constexpr uint32_t kA = 4 * MN;                                   // tensor memory: four accumulators, then A
-  constexpr uint32_t kTmemCols = kA + kDequantGroups * kTurn * 64 <= 256 ? 256 : 512;
+  constexpr uint32_t kTmemCols = kA + kDequantGroups * 64 <= 256 ? 256 : 512;       // 32 and 64 rows of x
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t s_ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint8_t* ring = smem_raw + (s_ring - smem_u32(smem_raw));
@@ -451,10 +448,10 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
       bool ok = true;
       RingAt at_ring{0, 0u};
       for (int it = 0; ok && it < n_it; ++it, at_ring.step(1, p.stages)) {
-        const int st = at_ring.st, turn = it / kTurn, buf = turn % kDequantGroups, part = it % kTurn;
+        const int st = at_ring.st, buf = it % kDequantGroups;
         ok = mbar_wait(full(st), at_ring.parity, abort_flag, kStatusTimeoutMma) &&
-             (part != 0 || mbar_wait(a_full(buf), (turn / kDequantGroups) & 1, abort_flag, kStatusTimeoutMma));
-        const uint32_t ta = tmem + kA + (buf * kTurn + part) * 64;
+             mbar_wait(a_full(buf), (it / kDequantGroups) & 1, abort_flag, kStatusTimeoutMma);
+        const uint32_t ta = tmem + kA + buf * 64;
         const uint64_t bd = make_kmajor_desc(s_ring + static_cast<uint32_t>(st) * stage_bytes, 128);
         for (int g = 0; ok && g < SG; ++g) {
           const int q = it * SG + g, d = q & 3;
@@ -470,7 +467,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
           umma_commit(d_full(d));
         }
         if (ok) {
-          if (part == kTurn - 1 || it + 1 == n_it) umma_commit(a_empty(buf));
+          umma_commit(a_empty(buf));
           umma_commit(empty(st));
         }
       }
@@ -481,9 +478,8 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
     const int group = (warp - 8) >> 2, r16 = row & 15;
     bool ok = true;
     RingAt at_ring{0, 0u};
-    at_ring.step(group * kTurn, p.stages);
-    for (int it0 = group * kTurn, round = 0; ok && it0 < n_it; it0 += kDequantGroups * kTurn, ++round) {
-     for (int it = it0; ok && it < min(it0 + kTurn, n_it); ++it) {
+    at_ring.step(group, p.stages);
+    for (int it = group, round = 0; ok && it < n_it; it += kDequantGroups, ++round) {
       const int st = at_ring.st;
       ok = mbar_wait_warp(full(st), at_ring.parity, abort_flag, kStatusTimeoutProducer);
       if (!ok) break;
@@ -496,8 +492,8 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
       if (has_zeros) z = load_zeros<SG>(stage + kX + kW + 128 * scale_row + row * kZeroRow);
       __syncwarp();
       if (lane == 0) mbar_arrive(empty(st));
-      at_ring.step(1, p.stages);
-      if (it == it0 && round > 0) ok = mbar_wait_warp(a_empty(group), (round - 1) & 1, abort_flag, kStatusTimeoutMma);
+      at_ring.step(kDequantGroups, p.stages);
+      if (round > 0) ok = mbar_wait_warp(a_empty(group), (round - 1) & 1, abort_flag, kStatusTimeoutMma);
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
@@ -523,11 +519,8 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
             }
           }
         }
-        tmem_st_32x32(tmem + lanes + kA + (group * kTurn + it - it0) * 64 + half * 32, o);
+        tmem_st_32x32(tmem + lanes + kA + group * 64 + half * 32, o);
       }
-     }
-      if (!ok) break;
-      at_ring.step(kTurn, p.stages);                                // the other group's turn
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -557,20 +550,13 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const Int4Params p) {
         ok = mbar_wait_warp(d_full(d), (q >> 2) & 1, abort_flag, kStatusTimeoutMma);
         if (!ok) break;
         tc_fence_after();
-        if (MN == 16) {
-          uint32_t v[16];
-          tmem_ld_32x16_wait(tmem + lanes + d * MN, v);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[i] = fmaf(__uint_as_float(v[i]), s[g], acc[i]);
-        } else {
+        for (int c = 0; c < MN / 32; ++c) {
+          uint32_t v[32];
+          tmem_ld_32x32(tmem + lanes + d * MN + c * 32, v);
+          tmem_ld_wait_dep(v);
 #pragma unroll
-          for (int c = 0; c < MN / 32; ++c) {
-            uint32_t v[32];
-            tmem_ld_32x32(tmem + lanes + d * MN + c * 32, v);
-            tmem_ld_wait_dep(v);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) acc[(c * 32 + i) % MN] = fmaf(__uint_as_float(v[i]), s[g], acc[(c * 32 + i) % MN]);
-          }
+          for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(v[i]), s[g], acc[c * 32 + i]);
         }
         tc_fence_before();
         __syncwarp();
@@ -625,11 +611,7 @@ typedef void (*Int4Tile)(const CUtensorMap, const Int4Params);
 
 template <bool BF16, int SG>
 Int4Tile pick_tile_rows(int mn) {
-  switch (mn) {
-    case 16: return int4_tile_kernel<BF16, SG, 16>;
-    case 32: return int4_tile_kernel<BF16, SG, 32>;
-    default: return int4_tile_kernel<BF16, SG, 64>;
-  }
+  return mn == 32 ? int4_tile_kernel<BF16, SG, 32> : int4_tile_kernel<BF16, SG, 64>;
 }
 template <bool BF16>
 Int4Tile pick_tile(int sg, int mn) {
@@ -781,7 +763,7 @@ FDB_API void* fdb_int4_linear_create(const Int4Desc* d) {
     }
   } else {
     const int mn = d->tile_rows;
-    if ((mn != 16 && mn != 32 && mn != 64) || d->splits < 1 || d->splits > 8 || d->splits > p.k_tiles) {
+    if ((mn != 32 && mn != 64) || d->splits < 1 || d->splits > 8 || d->splits > p.k_tiles) {
       delete op; return fail("bad tile form");
     }
     p.splits = d->splits;

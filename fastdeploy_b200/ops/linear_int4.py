@@ -133,8 +133,10 @@ def pack_linear_weight_int4(qweight: torch.Tensor, scales: torch.Tensor, zero_po
     return Int4Weight(data, s.dtype, z is not None, n, k, group)
 
 
-# Up to this many rows of x the vector kernel is the faster one: 16 rows of 4096 x 4096 take it 12 us and the tensor-core
-# kernel 16, of 28672 x 8192 68 and 70; 32 rows 115 and 74.
+# Up to this many rows of x take the vector kernel, whose CTAs of 16 weight rows each read x again; more the tensor-core kernel,
+# whose blocks cost the same up to 32 rows. Microseconds of both, fp16, at 16 and at 17 rows: 28672 x 8192 64 and 68, then 96
+# and 68; 14336 x 8192 39 and 37, then 53 and 37; 9472 x 4096 16 and 20, then 25 and 20; 4096 x 4096 12 and 16, then 14 and 16.
+# Weights of a few MB would keep the vector kernel a little longer (768 x 768 at 32 rows: 6 and 12).
 VECTOR_ROWS = 16
 
 
@@ -142,7 +144,7 @@ def _tile_form(m: int, weight: Int4Weight, sms: int) -> Tuple[int, int]:
     """(rows of x per tile, splits of K) of the tensor-core kernel, (0, 1) for the vector kernel."""
     if m <= VECTOR_ROWS:
         return 0, 1
-    rows = 16 if m <= 16 else 32 if m <= 32 else 64
+    rows = 32 if m <= 32 else 64
     ctas, k_tiles = -(-weight.n // 128) * -(-m // rows), -(-weight.k // 128)
     return rows, max(1, min(8, sms // ctas, k_tiles // 4))
 
