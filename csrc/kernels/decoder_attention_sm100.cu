@@ -22,15 +22,17 @@
 // are held 2^7 times as large (at most 2^15): below 2^-21 a weight is off by at most 2^-32, all of up to 2^20 keys together by
 // 2^-12 of the largest. l and O carry the same factor, which the quotient does not see.
 //
-// One 16384-token causal sequence, 16 query heads over 4 of 128 columns, bf16: 1054 us, 1.04 PFLOP/s (1.4 is what a long
-// cuBLAS product sustains). A pair of tiles takes 3500 clocks a key tile where the products need 2048 and the exponential
-// unit 2048: what is left is the chain S -> maximum -> exponentials -> P of one tile, which only the other tile overlaps.
-// A quarter of the exponentials as a polynomial on the FMA pipe was slower (1109 us: spilled registers). Short sequences
-// are bound by a CTA's start (prologue and first copies, 10000 clocks): 64 of 16 to 512 tokens, 12 heads of 64, 84 us.
+// One 16384-token causal sequence, 16 query heads over 4 of 128 columns, bf16: 1070 us, 1.03 PFLOP/s (1.4 is what a long
+// cuBLAS product sustains). A pair of tiles takes 3700 clocks a key tile where the products need 2048 and the exponential
+// unit 2048 (either pipe 55 % busy): what is left is the chain S -> maximum -> exponentials -> P of one tile, which only the
+// other tile overlaps. A quarter of the exponentials as a polynomial on the FMA pipe was slower (1109 us: spilled registers).
+// Short sequences are bound by a CTA's start and end (64 of 16 to 512 tokens, 12 heads of 64: 82 us, 13600 clocks a CTA with
+// every pipe under 20 %).
 //
 // own_keys_kernel: an item's own keys are met by its G query rows alone, so that part is bound by the bytes of K and V;
 // it brings them through a cp.async ring to the fragments of mma.sync and joins the two parts. 64 items, 4096 shared and 1
-// to 512 own keys, 8 key heads of 128: 42 us, 128 items, 32768 shared and 64 to 1024 own keys: 154 us (2.7 TB/s).
+// to 512 own keys, 8 key heads of 128: 40 us, 128 items, 32768 shared and 64 to 1024 own keys: 157 us (the prefix 80, the own
+// keys 72 at 3.9 TB/s).
 //
 // Every wait is bounded and reports through the status word.
 #include "fdb_common.h"

@@ -9,8 +9,9 @@
 // summed on their own in fp32 and multiplied by the scale in fp32: no rounding before the output's.
 //
 // The warps of a CTA share 16 weight rows and split K; their sums meet in shared memory in a fixed order. One row of x,
-// 28672 x 8192, groups of 128, fp16: 33 us, 3.7 TB/s; bound by the ALU pipe (an AND-OR or a shift is half rate: five a word
-// of eight weights in fp16, seven in bf16, 71 % busy), not by DRAM (57 %).
+// 28672 x 8192, groups of 128, fp16: 33 us, 3.7 TB/s, 57 % of a copy's bandwidth; the ALU pipe (an AND-OR or a shift is half
+// rate: five a word of eight weights in fp16, seven in bf16) is 64 % busy, and warps wait for it and for issue slots before
+// they wait for DRAM.
 #include "fdb_common.h"
 #include "sm100_ptx.cuh"
 
@@ -358,8 +359,9 @@ int4_linear_kernel(const Int4Params p) {
 //   MMA         one product per scale group into one of four accumulators in tensor memory
 //   drain       four warps, a weight row per thread: sum += scale * accumulator, in fp32
 // so that the scales meet fp32 sums here too and the two kernels differ only in the order of their additions. 64 rows,
-// 14336 x 8192, bf16 with zero points: 39 us, about 1000 clocks a block on 112 SMs, bound by the unpacking. Few weight
-// rows: up to eight CTAs of a cluster split K and add their sums, in their order, over distributed shared memory.
+// 14336 x 8192, bf16 with zero points: 39 us, 1030 clocks a block on 112 SMs, in which the ALU pipe (the unpacking) is 60 %
+// busy and the tensor pipe 25 %; the rest is waiting between the roles. Few weight rows: up to eight CTAs of a cluster split
+// K and add their sums, in their order, over distributed shared memory.
 constexpr int kTileThreads = 512;
 constexpr int kDequantGroups = 2;
 constexpr int kMaxInt4Stages = 8;
