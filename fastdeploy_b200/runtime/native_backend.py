@@ -1239,8 +1239,12 @@ def _lower_standard_attention(self: Lowering, node: Node):
         b, heads, s, d = shapes[0]
         kv_heads = shapes[1][1]
         kv = [b, kv_heads, s, d]
+    if b * s * d < 1:
+        return False
     scale = float(node.attr("scale", 1.0 / math.sqrt(d)))
-    if shapes[1] != kv or shapes[2] != kv or d % 8 or d > 128 or heads % kv_heads or heads // kv_heads > 128 or scale <= 0:
+    if shapes[1] != kv or shapes[2] != kv or d % 8 or d > 128 or heads % kv_heads or heads // kv_heads > 128:
+        return False
+    if not 0.0 < scale < math.inf:
         return False
 
     def rows(name, n):
@@ -1277,9 +1281,9 @@ def _lower_MatMulNBits(self: Lowering, node: Node):
     if ins[5] and ins[5] not in inits:
         return False
     shp = self.info.shapes[ins[0]]
-    if shp[-1] != k:
-        return False
     rows, groups = _rows_of(shp), -(-k // group)
+    if shp[-1] != k or len(shp) < 2 or rows < 1:
+        return False
     # nodes may share the weight and differ in all that is packed with it
     key = (*ins[1:4], n, k, group, "int4")
     if key not in self.packed:

@@ -94,3 +94,19 @@ def test_a_computed_bias_is_left_to_the_interpreter(recorded):
         g.add_node("MatMulNBits", ins, [f"y{i}"], domain="com.microsoft", N=N, K=K, bits=4, block_size=32)
     results, products, _ = recorded(g, {"x": [3, K]})
     assert results == [None, False] and len(products) == 1
+
+
+@pytest.mark.parametrize("shape", [[K], [0, K], [2, 0, K]])
+def test_vectors_and_empty_inputs_are_left_to_the_interpreter(recorded, shape):
+    results, products, _ = recorded(shared_weight_graph((1.0, None, 32)), {"x": shape})
+    assert results == [False] and not products
+
+
+@pytest.mark.parametrize("shape", [[0, 5, 16], [2, 0, 16]])
+@pytest.mark.parametrize("scale", [0.25, None])
+def test_empty_attention_and_odd_scales_are_left_to_the_interpreter(shape, scale):
+    for value in ([scale] if scale else [float("nan"), float("inf"), 0.0, -1.0]):
+        g = Graph("m", 23)
+        g.add_node("Attention", ["q", "k", "v"], ["y"], q_num_heads=2, kv_num_heads=2, scale=value)
+        rec = Recorder(g, dict.fromkeys("qkv", shape if scale else [2, 5, 16]))
+        assert native_backend._lower_standard_attention(rec, g.nodes[0]) is False
