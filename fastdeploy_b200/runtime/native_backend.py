@@ -1220,6 +1220,16 @@ def _lower_EmbedLayerNorm(self: Lowering, node: Node):
     self.vals[node.outputs[0]] = Val(y.unflatten(0, out_shape[:-1]), False)
 
 
+def _separate_rows(self: Lowering, name: str, rows: int, cols: int, node: Node) -> torch.Tensor:
+    """``rows_view`` of rows that do not share memory (those of an expanded value do)."""
+    t = self.rows_view(name, rows, cols)
+    if rows == 1 or t.stride(0) >= cols:
+        return t
+    dst = torch.zeros(rows, cols, dtype=self.dtype, device=self.device)
+    self.copy(t, dst, f"to_rows({name})", node)
+    return dst
+
+
 def _lower_standard_attention(self: Lowering, node: Node):
     """The standard ONNX operator over whole prompts, ``[B, S, heads * D]`` or ``[B, heads, S, D]``: every batch item is
     a sequence of the packed kernel (ops/decoder.py). Masks, past keys, further outputs and a soft cap run elsewhere."""
@@ -1249,7 +1259,7 @@ def _lower_standard_attention(self: Lowering, node: Node):
 
     def rows(name, n):
         if flat:
-            return self.rows_view(name, b * s, n * d)
+            return _separate_rows(self, name, b * s, n * d, node)
         buf = torch.zeros(b * s, n * d, dtype=self.dtype, device=self.device)
         self.copy(self.as_torch(name), buf.view(b, s, n, d).permute(0, 2, 1, 3), f"rows({name})", node)
         return buf
@@ -1293,7 +1303,7 @@ def _lower_MatMulNBits(self: Lowering, node: Node):
         self.packed[key] = pack_linear_weight_int4(
             torch.from_numpy(np.ascontiguousarray(inits[ins[1]])).view(n, groups, group // 2).to(self.device),
             scales.to(self.device), zeros, k=k)
-    x2 = self.rows_view(ins[0], rows, k)
+    x2 = _separate_rows(self, ins[0], rows, k, node)
     bias = self.const_f32(ins[5]).float().reshape(-1).contiguous() if ins[5] else None
     y = torch.zeros(rows, _round8(n), dtype=self.dtype, device=self.device)
     op = Int4Linear(x2, self.packed[key], y[:, :n], bias=bias, status=self.plan.status, name=f"int4:{node.name}")

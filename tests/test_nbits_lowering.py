@@ -102,6 +102,19 @@ def test_vectors_and_empty_inputs_are_left_to_the_interpreter(recorded, shape):
     assert results == [False] and not products
 
 
+def test_broadcast_rows_are_copied_apart(monkeypatch, recorded):
+    """An Expand is a view whose rows share memory; the product wants them one behind the other."""
+    from fastdeploy_b200.ops import linear_int4
+    seen = []
+    row = torch.arange(K).to(torch.float16)
+    product = linear_int4.Int4Linear
+    monkeypatch.setattr(linear_int4, "Int4Linear", lambda x, *a, **kw: seen.append(x.clone()) or seen.append(x.stride(0)) or product(x, *a, **kw))
+    monkeypatch.setattr(Recorder, "rows_view", lambda self, name, rows, cols: row.expand(rows, cols))
+    monkeypatch.setattr(Recorder, "copy", lambda self, src, dst, *a: dst.copy_(src), raising=False)
+    results, _, _ = recorded(shared_weight_graph((1.0, None, 32)), {"x": [5, K]})
+    assert results == [None] and torch.equal(seen[0], row.expand(5, K)) and seen[1] >= K
+
+
 @pytest.mark.parametrize("shape", [[0, 5, 16], [2, 0, 16]])
 @pytest.mark.parametrize("scale", [0.25, None])
 def test_empty_attention_and_odd_scales_are_left_to_the_interpreter(shape, scale):

@@ -54,3 +54,43 @@ def test_nodes_with_one_weight_and_a_computed_bias(rows):
         got = plan.outputs[name].logical().double().cpu().numpy()
         tol = k * 2.0 ** -23 * a + 2.0 ** -11 * (np.abs(y) + (3 * a + np.abs(y) if name == "y4" else 0)) + 2.0 ** -24
         assert (np.abs(got - y) <= tol).all(), (name, np.abs(got - y).max())
+
+
+def test_expanded_values_feed_the_operators():
+    """Rows that an Expand makes share memory; results are those of the graph with the values written out, bit for bit."""
+    from fastdeploy_b200.ir.graph import Graph
+    from fastdeploy_b200.runtime.native_backend import build_plan
+    rng = np.random.default_rng(1)
+    b, n, k, group, d = 5, 32, 64, 32, 16
+    w = rng.integers(0, 256, (n, k // 2)).astype(np.uint8)
+    s = (rng.integers(1, 65, (n, k // group)) / 1024).astype(np.float32)
+    x, y = rng.standard_normal((1, 1, k)).astype(np.float32), rng.standard_normal((b, 1, n)).astype(np.float32)
+    outs = []
+    for expand in (True, False):
+        g = Graph("m", 23)
+        g.add_input("x", "float32", [1 if expand else b, 1, k])
+        g.add_input("q", "float32", [b, 1, n])
+        g.add_initializer("w", w), g.add_initializer("s", s)
+        name = "x"
+        if expand:
+            g.add_node("Cast", ["x"], ["x16"], to=10)
+            g.add_node("Expand", ["x16", g.add_initializer("shape", np.array([b, 1, k], np.int64))], ["wide"])
+            name = "wide"
+        g.add_node("MatMulNBits", [name, "w", "s"], ["p"], domain="com.microsoft", N=n, K=k, bits=4, block_size=group)
+        kv = name
+        g.add_node("Slice", [name] + [g.add_initializer(f"c{i}", np.array([v], np.int64)) for i, v in enumerate((0, n, 2))], ["kv"])
+        kv = "kv"
+        g.add_node("Attention", ["q", kv, kv], ["a"], q_num_heads=n // d, kv_num_heads=n // d)
+        for o in "pa":
+            g.add_output(o, "float32", [b, 1, n])
+        plan = build_plan(g, {"x": [1 if expand else b, 1, k], "q": [b, 1, n]}, "cuda:0")
+        names = [st.name for st in plan.steps]
+        assert any(m.startswith("int4") for m in names) and "causal_attention" in names
+        plan.inputs["x"].t.copy_(torch.from_numpy(x if expand else np.repeat(x, b, 0)))
+        plan.inputs["q"].t.copy_(torch.from_numpy(y))
+        plan.run()
+        torch.cuda.synchronize()
+        plan.status.check()
+        outs.append({o: plan.outputs[o].logical().float().cpu() for o in "pa"})
+    assert all(torch.equal(outs[0][o], outs[1][o]) for o in "pa")
+    assert outs[0]["p"].abs().max() > 0 and outs[0]["a"].abs().max() > 0
